@@ -424,6 +424,139 @@ B2G_API b2g_status b2g_probe_mma(b2g_handle* h, const b2g_probe_desc* p, uint64_
 B2G_API b2g_status b2g_trace_enable(b2g_handle* h, int max_ctas);
 B2G_API b2g_status b2g_trace_read(const b2g_handle* h, uint32_t* out, int nwords);
 
+/* ------------------------------------------------------------------------------
+ * Operators around a linear layer of a language model (no counterpart in the
+ * reference, which has no model): microscaled casts of activations, weights and
+ * gradients; the norms, gate and residual addition before and after a block; and
+ * the product of a few tokens with microscaled weights.  Formats: B2G_FMT_NVFP4,
+ * B2G_FMT_MXF4 and B2G_FMT_MXF8, in the layout b2g_gemm reads.  Matrices are
+ * row-major with a leading dimension in elements; elements of a row are contiguous.
+ * b2g_residual_norm_backward and b2g_linear use the handle's workspace: calls of one
+ * handle on different streams must not overlap.  A workspace grows on the first call
+ * that needs more (which synchronises the stream), so make such a call before a
+ * stream capture. */
+
+typedef enum b2g_dtype { B2G_F32 = 0, B2G_BF16 = 1, B2G_F16 = 2 } b2g_dtype;
+
+/* Casts in[rows][cols], times `scale`, to codes with one scale per block of 16
+ * (NVFP4: ue4m3, e4m3(amax/6)) or 32 (MX: E8M0) elements, by b2g_quantize's rules:
+ * along the rows (codes, sf) and, with codes_t and sf_t, along the columns in the same
+ * pass, which is the operand of the products that run over the rows (dw = dy^T . x).
+ * Either pair may be NULL.  With Kp = cols and Tp = rows rounded up to 32:
+ *   codes   [rows][Kp] elements (two e2m1 per byte, even index low; e4m3 bytes),
+ *   sf      [rows][Kp / block], codes_t [cols][Tp], sf_t [cols][Tp / block];
+ * padding holds zeros.  b2g_gemm takes them with K = Kp (Tp).  codes are 16-byte
+ * aligned; `in` needs the alignment of its elements only.
+ * rand NULL: to nearest even.  Else stochastic rounding: rand[rows][cols] holds one
+ * random byte r per element, used for both copies; with |x / s| = (n + f) steps of the
+ * element format the code is n + 1 steps where f + (r + 1/2) / 256 >= 1, else n.
+ * A block that holds an infinity or a NaN gets a NaN scale. */
+typedef struct b2g_block_quant_desc {
+  int32_t format;        /* B2G_FMT_NVFP4, B2G_FMT_MXF4, B2G_FMT_MXF8 */
+  int32_t in_type;       /* b2g_dtype */
+  int64_t rows, cols, ld_in;
+  const void* in;
+  void* codes;
+  void* sf;
+  void* codes_t;
+  void* sf_t;
+  const void* rand;      /* nullable */
+  int64_t ld_rand;
+  float scale;           /* > 0; its inverse goes into the product's alpha */
+  int32_t reserved;
+} b2g_block_quant_desc;
+B2G_API b2g_status b2g_block_quantize(b2g_handle* h, const b2g_block_quant_desc* d, void* stream);
+
+/* Reads codes and scales in b2g_block_quantize's layout back: out[rows][cols] =
+ * code * block scale * scale, rounded once to out_type. */
+B2G_API b2g_status b2g_block_dequantize(b2g_handle* h, int format, const void* d_codes,
+                                        const void* d_sf, int64_t rows, int64_t cols,
+                                        int out_type, void* d_out, int64_t ld_out, float scale,
+                                        void* stream);
+
+/* The step between two blocks of a residual network, one pass over the rows:
+ *   z = y * rstd(y) * w_post           (norm after a block; w_post NULL: z = y)
+ *   v = alpha * x + beta * gate * z    (gate NULL: 1; y NULL: v = alpha * x)
+ *   x_out = v                          (nullable)
+ *   h = v * rstd(v) * w_pre            (norm before the next; w_pre NULL: none)
+ * with rstd(a) = 1 / sqrt(mean(a^2) + eps) over the cols (at most 32768) of a row.
+ * h goes out in the operands' type (h), as codes and scales of h_format (codes, sf, in
+ * b2g_block_quantize's layout), or both.  gate has one row of cols (contiguous) for each
+ * rows_per_gate rows: 1 = one per token, rows = one for all, S = one per sequence of S.
+ * x, y, gate, w_post, w_pre, x_out and h have one type; rstd_post and rstd_pre (fp32
+ * [rows], nullable) are what the backward pass needs.  x_out may be x. */
+typedef struct b2g_residual_norm_desc {
+  int32_t type;          /* b2g_dtype */
+  int32_t h_format;      /* with codes and sf */
+  int64_t rows, cols;
+  int64_t ld_x, ld_y, ld_x_out, ld_h;
+  int64_t rows_per_gate;
+  const void* x;
+  const void* y;
+  const void* gate;
+  const void* w_post;
+  const void* w_pre;
+  void* x_out;
+  void* h;
+  void* codes;
+  void* sf;
+  float* rstd_post;
+  float* rstd_pre;
+  float eps, alpha, beta;
+  int32_t reserved;
+} b2g_residual_norm_desc;
+B2G_API b2g_status b2g_residual_norm(b2g_handle* h, const b2g_residual_norm_desc* d, void* stream);
+
+/* Its gradient.  In: dh (gradient of h, NULL: none) and dx_out (gradient of x_out that
+ * does not come through h, NULL: none), and of the forward pass x_out, y, gate, w_post,
+ * w_pre, rstd_post, rstd_pre (what it had; x_out, w_pre and rstd_pre only with dh).
+ * Out, each nullable: dx and dy in the operands' type; dgate fp32 [gates][cols], dw_post
+ * and dw_pre fp32 [cols], summed over the rows they were broadcast to, always in the
+ * same order. */
+typedef struct b2g_residual_norm_grad_desc {
+  int32_t type;          /* b2g_dtype */
+  int32_t reserved0;
+  int64_t rows, cols;
+  int64_t ld_dh, ld_dx_out, ld_x_out, ld_y, ld_dx, ld_dy;
+  int64_t rows_per_gate;
+  const void* dh;
+  const void* dx_out;
+  const void* x_out;
+  const void* y;
+  const void* gate;
+  const void* w_post;
+  const void* w_pre;
+  const float* rstd_post;
+  const float* rstd_pre;
+  void* dx;
+  void* dy;
+  float* dgate;
+  float* dw_post;
+  float* dw_pre;
+  float alpha, beta;
+} b2g_residual_norm_grad_desc;
+B2G_API b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_norm_grad_desc* d,
+                                              void* stream);
+
+/* out[T][N] = alpha * x[T][K] . W[N][K]^T for the few tokens of a decode step: x and
+ * out bf16 or fp16, W as codes and scales in b2g_block_quantize's layout ([N][Kp], Kp =
+ * K rounded up to 32, padding zero), x not cast: fp32 sums of products of x and the
+ * weights' values.  Reads the weights once for every 64 tokens; for many tokens cast x
+ * and use b2g_gemm.  w 16-byte, sfw 2-byte aligned. */
+typedef struct b2g_linear_desc {
+  int32_t format;        /* of W */
+  int32_t type;          /* of x and out: B2G_BF16 or B2G_F16 */
+  int64_t T, N, K;
+  int64_t ld_x, ld_out;
+  const void* x;
+  const void* w;
+  const void* sfw;
+  void* out;
+  float alpha;
+  int32_t reserved;
+} b2g_linear_desc;
+B2G_API b2g_status b2g_linear(b2g_handle* h, const b2g_linear_desc* d, void* stream);
+
 /* Descriptor encoders (host-side, no GPU needed), the engine's own encodings of
  * the bit layouts the reference builds at umma_tput.cu:147-156 and :190-255 and
  * tcgen05_sparse_mma.cu:191-228.  Exposed so tests can pin them. */

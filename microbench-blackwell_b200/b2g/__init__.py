@@ -15,21 +15,17 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
+from ._errors import B2GError
 from ._lib import (FMT_BF16, FMT_E2M1, FMT_E2M3, FMT_E3M2, FMT_E4M3, FMT_E5M2, FMT_F16,
                    FMT_MXF4, FMT_MXF8, FMT_NVFP4, FMT_S8, FMT_TF32, FMT_U8, GemmDesc,
                    ProbeDesc)
+from ._ops import LinearOps
 
 __all__ = [
     "B2GError", "Engine", "GemmDesc", "ProbeDesc", "plan_gemm",
     "FMT_BF16", "FMT_E4M3", "FMT_S8", "FMT_E2M1", "FMT_MXF8", "FMT_MXF4", "FMT_NVFP4",
     "FMT_TF32", "FMT_E5M2", "FMT_E2M3", "FMT_E3M2", "FMT_F16", "FMT_U8",
 ]
-
-
-class B2GError(RuntimeError):
-    def __init__(self, status: int, msg: str):
-        super().__init__(f"b2g status {status} ({_lib.STATUS.get(status, '?')}): {msg}")
-        self.status = status
 
 
 # bits per element of the packed formats whose tensors hold bytes
@@ -48,7 +44,7 @@ def _stream(stream) -> int:
     return int(stream.cuda_stream)
 
 
-class Engine:
+class Engine(LinearOps):
     """One handle of libb2g bound to one CUDA device."""
 
     def __init__(self, device: int = 0):

@@ -90,6 +90,59 @@ class ProbeDesc(C.Structure):
     ]
 
 
+# b2g_dtype
+F32 = 0
+BF16 = 1
+F16 = 2
+
+
+class BlockQuantDesc(C.Structure):
+    _fields_ = [
+        ("format", C.c_int32),
+        ("in_type", C.c_int32),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("ld_in", C.c_int64),
+        ("in", C.c_void_p),
+        ("codes", C.c_void_p),
+        ("sf", C.c_void_p),
+        ("codes_t", C.c_void_p),
+        ("sf_t", C.c_void_p),
+        ("rand", C.c_void_p),
+        ("ld_rand", C.c_int64),
+        ("scale", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+class ResidualNormDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("h_format", C.c_int32)] + [
+        (name, C.c_int64) for name in (
+            "rows", "cols", "ld_x", "ld_y", "ld_x_out", "ld_h", "rows_per_gate")] + [
+        (name, C.c_void_p) for name in (
+            "x", "y", "gate", "w_post", "w_pre", "x_out", "h", "codes", "sf", "rstd_post",
+            "rstd_pre")] + [
+        (name, C.c_float) for name in ("eps", "alpha", "beta")] + [("reserved", C.c_int32)]
+
+
+class ResidualNormGradDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("reserved0", C.c_int32)] + [
+        (name, C.c_int64) for name in (
+            "rows", "cols", "ld_dh", "ld_dx_out", "ld_x_out", "ld_y", "ld_dx", "ld_dy",
+            "rows_per_gate")] + [
+        (name, C.c_void_p) for name in (
+            "dh", "dx_out", "x_out", "y", "gate", "w_post", "w_pre", "rstd_post", "rstd_pre",
+            "dx", "dy", "dgate", "dw_post", "dw_pre")] + [
+        (name, C.c_float) for name in ("alpha", "beta")]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [("format", C.c_int32), ("type", C.c_int32)] + [
+        (name, C.c_int64) for name in ("T", "N", "K", "ld_x", "ld_out")] + [
+        (name, C.c_void_p) for name in ("x", "w", "sfw", "out")] + [
+        ("alpha", C.c_float), ("reserved", C.c_int32)]
+
+
 # (name, restype, argtypes) of every exported entry point of include/b2g.h
 _SIGS = [
     ("b2g_abi_version", C.c_int, []),
@@ -144,6 +197,14 @@ _SIGS = [
     ("b2g_sparse_meta_bytes", C.c_size_t, [C.c_int64, C.c_int64]),
     ("b2g_sparse_meta_prepare", C.c_int,
      [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
+    ("b2g_block_quantize", C.c_int, [C.c_void_p, C.POINTER(BlockQuantDesc), C.c_void_p]),
+    ("b2g_block_dequantize", C.c_int,
+     [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+      C.c_int64, C.c_float, C.c_void_p]),
+    ("b2g_residual_norm", C.c_int, [C.c_void_p, C.POINTER(ResidualNormDesc), C.c_void_p]),
+    ("b2g_residual_norm_backward", C.c_int,
+     [C.c_void_p, C.POINTER(ResidualNormGradDesc), C.c_void_p]),
+    ("b2g_linear", C.c_int, [C.c_void_p, C.POINTER(LinearDesc), C.c_void_p]),
     ("b2g_trace_enable", C.c_int, [C.c_void_p, C.c_int]),
     ("b2g_trace_read", C.c_int, [C.c_void_p, C.POINTER(C.c_uint32), C.c_int]),
     ("b2g_encode_idesc", C.c_uint32, [C.c_int] * 7),

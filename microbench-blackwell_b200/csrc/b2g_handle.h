@@ -1,0 +1,93 @@
+// b2g_handle.h -- the handle behind the C ABI and what its entry points share.  Not
+// part of the public ABI.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "b2g.h"
+
+typedef CUresult (*PFN_encodeTiled_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                      const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                      CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// b2g_gemm_host splits M into at most kHostChunks row chunks and N into at most
+// kHostColChunks column chunks
+constexpr int kHostChunks = 4;
+constexpr int kHostColChunks = 4;
+
+struct b2g_handle {
+  int device;
+  int sm_count;
+  int clock_khz;
+  int cc_major, cc_minor;
+  uint32_t* d_err;
+  PFN_encodeTiled_t encode_tiled;
+  void* ws;                // device workspace of b2g_gemm_host
+  size_t ws_bytes;
+  void* meta_ws;           // scratch: engine-layout 2:4 metadata of the last sparse call
+  size_t meta_ws_bytes;
+  void* sf_ws;             // scratch: engine-layout NVFP4 scale factors of the last call
+  size_t sf_ws_bytes;
+  void* d_probe;           // b2g_probe_mma result words
+  void* part_ws;           // split tail: fp32 partial tiles
+  size_t part_ws_bytes;
+  uint32_t* flag_ws;       // split tail: per-warp stamps (zeroed when allocated)
+  size_t flag_ws_bytes;
+  uint32_t epoch;          // stamp of the last split-tail launch
+  uint64_t wait_ns;        // limit of the kernel-side bounded waits (0: kWaitLimitNs)
+  // b2g_gemm_host pipeline: copy-in and copy-out streams, events per row chunk
+  cudaStream_t s_in, s_out;
+  cudaEvent_t ev_start, ev_out, ev_c, ev_a[kHostChunks], ev_b[kHostColChunks];
+  bool pipe_ready;
+  uint32_t* trace_host;    // host-mapped progress trace (nullable)
+  uint32_t* trace_dev;
+  int trace_ctas;
+  // co-resident cluster pairs per kernel instance and shared-memory size (the
+  // occupancy query of cta_group::2 launches), kept after the first query
+  struct OccEntry {
+    uint32_t key;
+    int smem, clusters;
+  } occ[16];
+  int n_occ;
+  // operators around the linear layer (op_api.cu): fp32 partial sums and laid-out
+  // operands of one call, and arrival counters that every launch leaves at zero
+  void* op_ws;
+  size_t op_ws_bytes;
+  uint32_t* op_count;
+  size_t op_count_words;
+  char last_error[512];
+};
+
+inline b2g_status fail(b2g_handle* h, b2g_status s, const char* fmt, ...) {
+  if (h) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(h->last_error, sizeof(h->last_error), fmt, ap);
+    va_end(ap);
+  }
+  return s;
+}
+
+#define B2G_CUDA(h, expr)                                                                  \
+  do {                                                                                     \
+    cudaError_t e__ = (expr);                                                              \
+    if (e__ != cudaSuccess)                                                                \
+      return fail((h), B2G_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__));     \
+  } while (0)
+
+// Make the handle's device current for the duration of a call.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) cudaSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    int cur;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};

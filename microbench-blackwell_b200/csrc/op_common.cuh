@@ -1,0 +1,285 @@
+// op_common.cuh -- device helpers of the operators around the linear layer: eight
+// elements at a time from 16- or 32-bit rows, and microscaled 4- and 8-bit codes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b2g {
+
+// Eight consecutive elements of a row as they lie in memory: one 16-byte word for
+// 16-bit types, two for fp32.
+template <typename T>
+struct Raw8 {
+  uint4 w[sizeof(T) == 4 ? 2 : 1];
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) {
+  return __bfloat162float(x);
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// Elements [0, n) of the eight at p, zeros after them; `vec`: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec) {
+  Raw8<T> r;
+  constexpr int W = sizeof(T) == 4 ? 2 : 1;
+  if (vec && n >= 8) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    return r;
+  }
+  uint32_t u[4 * W];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      u[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      const uint32_t lo = 2 * i < n ? __ldg(q + 2 * i) : 0u;
+      const uint32_t hi = 2 * i + 1 < n ? __ldg(q + 2 * i + 1) : 0u;
+      u[i] = lo | (hi << 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    r.w[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pair_f32(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t u[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w,
+                           r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = pair_f32<T>(u[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 b = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Stores the first n of eight values at p; `vec`: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool vec) {
+  if (vec && n >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = from_f32<T>(v[i]);
+}
+
+// ---------------------------------------------------------------- microscaled codes
+// Element formats with one scale per block (the numbers of BlockFmt are internal):
+//   NVFP4  e2m1, ue4m3 scale per 16:  s = e4m3(amax / 6)
+//   MXFP4  e2m1, E8M0 scale per 32:   s = 2^(floor(log2 amax) - 2)
+//   MXFP8  e4m3, E8M0 scale per 32:   s = 2^(floor(log2 amax) - 8)
+// codes = element(x / s), to nearest even and saturating.  A block that holds an
+// infinity or a NaN gets a NaN scale and so reads back as NaN: an overflow upstream
+// stays visible.
+enum BlockFmt : int { BF_NVFP4 = 0, BF_MXF4 = 1, BF_MXF8 = 2 };
+__host__ __device__ constexpr int bf_block(int f) { return f == BF_NVFP4 ? 16 : 32; }
+__host__ __device__ constexpr int bf_bits(int f) { return f == BF_MXF8 ? 8 : 4; }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// eight e2m1 codes, element i in bits [4i, 4i + 4)
+__device__ __forceinline__ uint32_t e2m1x8(const float (&x)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+  return r;
+}
+
+// values of eight e2m1 codes as fp16 pairs
+__device__ __forceinline__ void e2m1x8_pairs(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
+// value of the two e4m3 codes in the low bytes of w
+__device__ __forceinline__ float2 e4m3_pair(uint32_t w) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)w));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// 2^(byte - 127), the value of an E8M0 byte (255: NaN)
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7FFFFFFFu : byte << 23);
+}
+
+// The scale of a block from its largest magnitude: the stored byte, its value and
+// the reciprocal of the value (0 where all codes shall be 0).
+struct BlockScale {
+  uint32_t byte;
+  float value, inv;
+};
+
+template <int FMT>
+__device__ __forceinline__ BlockScale block_scale(float amax) {
+  BlockScale s;
+  const bool finite = amax < __uint_as_float(0x7F800000u);  // false for NaN too
+  if constexpr (FMT == BF_NVFP4) {
+    s.byte = e4m3x2(amax / 6.0f, 0.0f) & 0xFFu;
+    s.value = e4m3_pair(s.byte).x;
+    s.inv = s.byte ? __frcp_rn(s.value) : 0.0f;
+    if (!finite) s = {0x7Fu, 0.0f, 0.0f};
+  } else {
+    constexpr int emax = FMT == BF_MXF8 ? 8 : 2;
+    // exponent field of amax (0 for 0 and subnormals: their scale is clamped anyway)
+    const int e = (int)(__float_as_uint(amax) >> 23) - emax;
+    s.byte = e > 0 ? (uint32_t)e : 0u;
+    s.value = e8m0_value(s.byte);
+    s.inv = __uint_as_float((254u - s.byte) << 23);
+    if (!finite) s = {0xFFu, 0.0f, 0.0f};
+  }
+  return s;
+}
+
+// How x / s is formed.  MX scales are powers of two: x * (1 / s) is exact.  NVFP4:
+//   Q_DIVIDE  x / s rounded to fp32, right for any x;
+//   Q_SNAP    for x with at most 11 significant bits (16-bit inputs times a power of
+//             two).  The boundaries of e2m1 have at most 3 bits and s has 4, so x / s
+//             either lies on a boundary or at least 2^-13 beside it.  fma(x, 1/s, 48)
+//             - 48 rounds the quotient to a multiple of 2^-18: a quotient on a boundary
+//             comes out on it and no other crosses one, for two instructions where the
+//             division takes about ten.
+enum QuotientMode : int { Q_EXACT = 0, Q_DIVIDE = 1, Q_SNAP = 2 };
+
+template <int FMT, int QM>
+__device__ __forceinline__ float quotient(float x, const BlockScale& s) {
+  if constexpr (QM == Q_DIVIDE) return s.inv != 0.0f ? x / s.value : 0.0f;
+  if constexpr (QM == Q_SNAP) return __fadd_rn(__fmaf_rn(x, s.inv, 48.0f), -48.0f);
+  return __fmul_rn(x, s.inv);
+}
+
+// Stochastic rounding with a given byte r: |q| in steps of the element format goes up
+// when its fraction and (r + 1/2) / 256 together reach the next step.  Returns the
+// value on the format's grid.
+template <int FMT>
+__device__ __forceinline__ float round_stochastic(float q, uint32_t r) {
+  constexpr uint32_t low = FMT == BF_MXF8 ? 121u << 23 : 127u << 23;  // lowest binade
+  constexpr uint32_t mant = (FMT == BF_MXF8 ? 3u : 1u) << 23;
+  constexpr float top = FMT == BF_MXF8 ? 448.0f : 6.0f;
+  const float a = fabsf(q);
+  uint32_t e = __float_as_uint(a) & 0x7F800000u;
+  e = (e < low ? low : e) - mant;
+  const float step = __uint_as_float(e), inv = __uint_as_float((254u << 23) - e);
+  const float n = floorf(__fadd_rn(__fmul_rn(a, inv), __fmaf_rn((float)r, 0x1p-8f, 0x1p-9f)));
+  return copysignf(fminf(n * step, top), q);
+}
+
+// Q_SNAP's counterpart for stochastic rounding, whose thresholds have up to 12 bits:
+// x / s lies on a threshold or at least 2^-16 of itself beside it, so the quotient is
+// rounded to 20 significant bits.
+__device__ __forceinline__ float snap20(float q) {
+  return __uint_as_float((__float_as_uint(q) + 8u) & ~15u);
+}
+
+// Codes of eight elements of one block: 32 bits (e2m1) in w[0] or 64 (e4m3) in w[0..1].
+// rnd: eight random bytes, used when SR.
+template <int FMT, int QM, bool SR>
+__device__ __forceinline__ void encode8(const float (&x)[8], const BlockScale& s, uint2 rnd,
+                                        uint32_t (&w)[2]) {
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (SR) {
+      float t = QM == Q_DIVIDE ? quotient<FMT, Q_DIVIDE>(x[i], s) : __fmul_rn(x[i], s.inv);
+      if constexpr (QM == Q_SNAP) t = snap20(t);
+      q[i] = round_stochastic<FMT>(t, ((i < 4 ? rnd.x : rnd.y) >> (8 * (i & 3))) & 0xFFu);
+    } else {
+      q[i] = quotient<FMT, QM>(x[i], s);
+    }
+  }
+  if constexpr (FMT == BF_MXF8) {
+    w[0] = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
+    w[1] = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
+  } else {
+    w[0] = e2m1x8(q);
+    w[1] = 0u;
+  }
+}
+
+}  // namespace b2g

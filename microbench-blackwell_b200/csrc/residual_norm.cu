@@ -1,0 +1,438 @@
+// residual_norm.cu -- norms before and after a block, fused with its gate and residual
+// scale, and their gradient.
+//
+//   z = y * rstd(y) * w_post            (z = y without w_post)
+//   v = alpha * x + beta * gate * z     (v = alpha * x without y)
+//   x_out = v,  h = v * rstd(v) * w_pre,  rstd(a) = 1 / sqrt(mean(a^2) + eps)
+//
+// All sums and the row v are fp32; x_out and h are rounded once.  h is formed from the
+// unrounded v.
+#include "b2g.h"
+#include "op_common.cuh"
+#include "op_kernels.h"
+
+namespace b2g {
+namespace {
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+// Sums of K values over the CTA's row of threads (blockDim.x of them; one warp per row
+// where blockDim.x is 32).  `red`: K * 32 floats, not in use by an earlier call.
+template <int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if (blockDim.x == 32) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[k * 32 + warp] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? red[k * 32 + lane] : 0.0f);
+}
+
+// One row per blockDim.x threads, held in registers: NV times eight elements a thread.
+template <typename T, int NV, int HF>
+__global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormArgs a) {
+  __shared__ float red[2][32];
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= a.rows) return;  // whole warps: blockDim.y > 1 only with one warp per row
+  const bool vec = a.vec;
+  const int64_t width = HF < 0 ? a.cols : a.kp;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  const T* y = static_cast<const T*>(a.y) + row * a.ld_y;
+  Raw8<T> rx[NV], ry[NV];
+  int n[NV];
+  int64_t col[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    col[j] = ((int64_t)j * blockDim.x + threadIdx.x) * 8;
+    const int64_t left = a.cols - col[j];
+    n[j] = left < 0 ? 0 : left < 8 ? (int)left : 8;
+    rx[j] = load8(x + col[j], n[j], vec);
+    if (a.y) ry[j] = load8(y + col[j], n[j], vec);
+  }
+  float v[NV][8];
+  if (a.y) {
+    float r1 = 1.0f;
+    if (a.w_post) {
+      float ss[1] = {0.0f};
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float f[8];
+        unpack8(ry[j], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss[0] = fmaf(f[i], f[i], ss[0]);
+      }
+      row_sum(ss, red[0]);
+      r1 = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
+      if (a.rstd_post && threadIdx.x == 0) a.rstd_post[row] = r1;
+    }
+    const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float fx[8], fy[8];
+      unpack8(rx[j], fx);
+      unpack8(ry[j], fy);
+      if (a.w_post) {
+        float w[8];
+        unpack8(load8(static_cast<const T*>(a.w_post) + col[j], n[j], vec), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fy[i] = fy[i] * r1 * w[i];
+      }
+      if (gate) {
+        float g[8];
+        unpack8(load8(gate + col[j], n[j], vec), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) fy[i] *= g[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = fmaf(a.beta, fy[i], a.alpha * fx[i]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      unpack8(rx[j], v[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] *= a.alpha;
+    }
+  }
+  if (a.x_out) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      store8(static_cast<T*>(a.x_out) + row * a.ld_x_out + col[j], v[j], n[j], vec);
+  }
+  if (!a.w_pre) return;
+  float ss[1] = {0.0f};
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss[0] = fmaf(v[j][i], v[j][i], ss[0]);
+  row_sum(ss, red[1]);
+  const float r2 = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
+  if (a.rstd_pre && threadIdx.x == 0) a.rstd_pre[row] = r2;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float w[8];
+    unpack8(load8(static_cast<const T*>(a.w_pre) + col[j], n[j], vec), w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * r2 * w[i];
+    if (a.h) store8(static_cast<T*>(a.h) + row * a.ld_h + col[j], v[j], n[j], vec);
+    if constexpr (HF >= 0) {
+      constexpr int blk = bf_block(HF), bits = bf_bits(HF);
+      float amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[j][i]));
+      amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+      if constexpr (blk == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+      const BlockScale s = block_scale<HF>(amax);
+      uint32_t q[2];
+      encode8<HF, HF == BF_NVFP4 ? Q_DIVIDE : Q_EXACT, false>(v[j], s, make_uint2(0, 0), q);
+      if (col[j] < width) {
+        const int64_t e = row * a.kp + col[j];
+        if constexpr (HF == BF_MXF8)
+          *reinterpret_cast<uint2*>(a.codes + e) = make_uint2(q[0], q[1]);
+        else
+          *reinterpret_cast<uint32_t*>(a.codes + e * bits / 8) = q[0];
+        if ((threadIdx.x & (blk / 8 - 1)) == 0) a.sf[e / blk] = (uint8_t)s.byte;
+      }
+    }
+  }
+}
+
+template <typename T, int HF>
+cudaError_t norm_launch(const ResidualNormArgs& a, int sm_count, cudaStream_t s) {
+  const int64_t v = ((HF < 0 ? a.cols : a.kp) + 7) / 8;
+  // few rows: as many threads to a row as it has eights, for latency; many: four eights
+  // a thread, which keeps eight 16-byte loads in flight in each
+  const int want = a.rows < 2 * sm_count ? 1 : 4;
+  int nv = 1;
+  while (nv < 4 && (nv < want || (v + nv - 1) / nv > 1024)) nv *= 2;
+  int64_t tpr = ((v + nv - 1) / nv + 31) / 32 * 32;
+  if (tpr < 32) tpr = 32;
+  const int rpc = tpr == 32 ? 4 : 1;
+  const dim3 block((unsigned)tpr, rpc);
+  const unsigned grid = (unsigned)((a.rows + rpc - 1) / rpc);
+  if (nv == 1)
+    residual_norm_kernel<T, 1, HF><<<grid, block, 0, s>>>(a);
+  else if (nv == 2)
+    residual_norm_kernel<T, 2, HF><<<grid, block, 0, s>>>(a);
+  else
+    residual_norm_kernel<T, 4, HF><<<grid, block, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t norm_fmt(int h_fmt, const ResidualNormArgs& a, int sm_count, cudaStream_t s) {
+  switch (h_fmt) {
+    case BF_NVFP4: return norm_launch<T, BF_NVFP4>(a, sm_count, s);
+    case BF_MXF4: return norm_launch<T, BF_MXF4>(a, sm_count, s);
+    case BF_MXF8: return norm_launch<T, BF_MXF8>(a, sm_count, s);
+    default: return norm_launch<T, -1>(a, sm_count, s);
+  }
+}
+
+// ------------------------------------------------------------------ gradient
+// With v^ = v r2, y^ = y r1, p = w_pre dh, q = beta w_post g:
+//   dv = dx_out + r2 (p - v^ mean(p v^)),  dx = alpha dv,  dw_pre = sum dh v^
+//   dy = r1 (q dv - y^ mean(q dv y^)),  dgate = beta sum z dv,  dw_post = sum beta g dv y^
+// mean(q dv y^) follows from sums that need no dv: with A = sum p v, B = sum q y
+// (dx_out + r2 p), C = sum q y v it is r1 (B - r2^3 A C / D) / D.  So one reduction per
+// row gives both means.
+
+// Row means: stat[row] = {r2^3 A / D, r1^3 (B - r2^3 (A / D) C) / D} (the second r1-free
+// without w_post: 0).
+template <typename T>
+__global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradArgs a, float2* stat) {
+  __shared__ float red[3 * 32];
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= a.rows) return;
+  const bool vec = a.vec;
+  const float r2 = a.dh ? a.rstd_pre[row] : 0.0f;
+  const float r1 = a.w_post ? a.rstd_post[row] : 0.0f;
+  const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
+  float s[3] = {0.0f, 0.0f, 0.0f};
+  for (int64_t c = threadIdx.x * 8; c < a.cols; c += blockDim.x * 8) {
+    const int n = a.cols - c < 8 ? (int)(a.cols - c) : 8;
+    float p[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (a.dh) {
+      float w[8];
+      unpack8(load8(static_cast<const T*>(a.dh) + row * a.ld_dh + c, n, vec), p);
+      unpack8(load8(static_cast<const T*>(a.v) + row * a.ld_v + c, n, vec), v);
+      unpack8(load8(static_cast<const T*>(a.w_pre) + c, n, vec), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] *= w[i];
+        s[0] = fmaf(p[i], v[i], s[0]);
+      }
+    }
+    if (a.w_post) {
+      float y[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      unpack8(load8(static_cast<const T*>(a.y) + row * a.ld_y + c, n, vec), y);
+      unpack8(load8(static_cast<const T*>(a.w_post) + c, n, vec), w);
+      if (a.dx_out) unpack8(load8(static_cast<const T*>(a.dx_out) + row * a.ld_dx_out + c, n, vec), d);
+      if (gate) {
+        float g[8];
+        unpack8(load8(gate + c, n, vec), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] *= g[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float qy = w[i] * y[i];
+        s[1] = fmaf(qy, fmaf(r2, p[i], d[i]), s[1]);
+        s[2] = fmaf(qy, v[i], s[2]);
+      }
+    }
+  }
+  row_sum(s, red);
+  if (threadIdx.x == 0) {
+    const float m = 1.0f / (float)a.cols;
+    const float c2 = r2 * r2 * r2 * s[0] * m;
+    stat[row] = make_float2(c2, r1 * r1 * r1 * a.beta * (s[1] - c2 * s[2]) * m);
+  }
+}
+
+// How the column pass cuts the rows: a chunk of whole gates (their dgate rows are then
+// written directly) where a gate has few rows, else chunks within one gate.
+struct GradChunks {
+  bool whole;         // a chunk holds whole gates
+  int64_t per;        // rows of a gate (all rows without one)
+  int64_t gates;
+  int64_t rows;       // rows of a chunk (whole: a multiple of per)
+  int64_t per_gate;   // chunks of a gate (whole: unused)
+  int64_t chunks;
+};
+constexpr int kLanes = 8;       // rows a column CTA works on at once
+constexpr int kGradCols = 256;  // columns of a column CTA
+
+GradChunks grad_chunks(const ResidualNormGradArgs& a, int sm_count) {
+  GradChunks c;
+  c.per = a.gate && a.rows_per_gate < a.rows ? a.rows_per_gate : a.rows;
+  c.gates = (a.rows + c.per - 1) / c.per;
+  // chunks of 16 to 128 rows, about four CTAs an SM
+  const int64_t col_tiles = (a.cols + kGradCols - 1) / kGradCols;
+  int64_t r = a.rows * col_tiles / (4 * (int64_t)sm_count);
+  r = r < 16 ? 16 : r > 128 ? 128 : r;
+  c.whole = c.gates > 1 && c.per <= r;
+  if (c.whole) {
+    c.rows = r / c.per * c.per;
+    c.per_gate = 0;
+    c.chunks = (a.rows + c.rows - 1) / c.rows;
+  } else {
+    c.rows = r;
+    c.per_gate = (c.per + r - 1) / r;
+    c.chunks = c.gates * c.per_gate;
+  }
+  return c;
+}
+
+// Column pass: 256 columns (eight a thread) of one chunk of rows, a row per warp.  Sums
+// over the chunk go to part[chunk][3][cols] (dw_pre, dw_post, dgate).
+template <typename T>
+__global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradArgs a, GradChunks ck,
+                                                        const float2* stat, float* part) {
+  __shared__ float red[kLanes][kGradCols];
+  const int lane = threadIdx.x, ry = threadIdx.y;
+  const int64_t chunk = blockIdx.x;
+  const int64_t c = (int64_t)blockIdx.y * kGradCols + lane * 8;
+  const int n = c >= a.cols ? 0 : a.cols - c < 8 ? (int)(a.cols - c) : 8;
+  const bool vec = a.vec;
+  int64_t r0, r1;
+  if (ck.whole) {
+    r0 = chunk * ck.rows;
+    r1 = r0 + ck.rows;
+  } else {
+    const int64_t g = chunk / ck.per_gate;
+    r0 = g * ck.per + chunk % ck.per_gate * ck.rows;
+    r1 = r0 + ck.rows < (g + 1) * ck.per ? r0 + ck.rows : (g + 1) * ck.per;
+  }
+  if (r1 > a.rows) r1 = a.rows;
+  float wq[8], wp[8], g[8];
+  if (a.w_post) unpack8(load8(static_cast<const T*>(a.w_post) + c, n, vec), wp);
+  if (a.dh) unpack8(load8(static_cast<const T*>(a.w_pre) + c, n, vec), wq);
+  float dwq[8], dwp[8], dg[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    dwq[i] = dwp[i] = dg[i] = 0.0f;
+    g[i] = 1.0f;
+    if (!a.w_post) wp[i] = 1.0f;
+    if (!a.dh) wq[i] = 0.0f;
+  }
+  // rows of this thread: whole gates in turn, or every kLanes-th row of the chunk
+  const int64_t run = ck.whole ? ck.per : 1;
+  for (int64_t rb = r0 + ry * run; rb < r1; rb += kLanes * run) {
+    const int64_t re = rb + run < r1 ? rb + run : r1;
+    if (a.gate && (ck.whole || rb == r0 + ry * run))
+      unpack8(load8(static_cast<const T*>(a.gate) + rb / ck.per * a.cols + c, n, vec), g);
+    for (int64_t r = rb; r < re; ++r) {
+      const float2 st = stat[r];
+      float dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (a.dx_out) unpack8(load8(static_cast<const T*>(a.dx_out) + r * a.ld_dx_out + c, n, vec), dv);
+      if (a.dh) {
+        const float r2 = a.rstd_pre[r];
+        float dh[8], v[8];
+        unpack8(load8(static_cast<const T*>(a.dh) + r * a.ld_dh + c, n, vec), dh);
+        unpack8(load8(static_cast<const T*>(a.v) + r * a.ld_v + c, n, vec), v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dv[i] += r2 * wq[i] * dh[i] - v[i] * st.x;
+          dwq[i] = fmaf(dh[i], v[i] * r2, dwq[i]);
+        }
+      }
+      float o[8];
+      if (a.dx) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = a.alpha * dv[i];
+        store8(static_cast<T*>(a.dx) + r * a.ld_dx + c, o, n, vec);
+      }
+      if (a.y) {
+        const float r1s = a.w_post ? a.rstd_post[r] : 1.0f;
+        float y[8];
+        unpack8(load8(static_cast<const T*>(a.y) + r * a.ld_y + c, n, vec), y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float bd = a.beta * dv[i], yh = y[i] * r1s, dz = bd * g[i];
+          dg[i] = fmaf(bd * wp[i], yh, dg[i]);
+          dwp[i] = fmaf(dz, yh, dwp[i]);
+          o[i] = r1s * wp[i] * dz - y[i] * st.y;
+        }
+        if (a.dy) store8(static_cast<T*>(a.dy) + r * a.ld_dy + c, o, n, vec);
+      }
+    }
+    if (ck.whole && a.dgate) {
+      store8(a.dgate + rb / ck.per * a.cols + c, dg, n, false);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dg[i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float(&acc)[8] = k == 0 ? dwq : k == 1 ? dwp : dg;
+    const bool on = k == 0 ? a.dw_pre != nullptr : k == 1 ? a.dw_post != nullptr
+                                                          : a.dgate != nullptr && !ck.whole;
+    if (!on) continue;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[ry][lane * 8 + i] = acc[i];
+    __syncthreads();
+    const int t = ry * 32 + lane;
+    float sum = 0.0f;
+#pragma unroll
+    for (int l = 0; l < kLanes; ++l) sum += red[l][t];
+    const int64_t cc = (int64_t)blockIdx.y * kGradCols + t;
+    if (cc < a.cols) part[(chunk * 3 + k) * a.cols + cc] = sum;
+  }
+}
+
+// out[g][c] = sum of count rows of part (stride row_stride floats) from row first + g *
+// count on, for 32 columns of one g: 32 threads along the columns, 8 down the rows.
+__global__ void __launch_bounds__(256) grad_sum_kernel(const float* part, int64_t row_stride,
+                                                       int64_t count, int64_t cols, float* out) {
+  __shared__ float red[8][32];
+  const int64_t c = (int64_t)blockIdx.y * 32 + threadIdx.x, g = blockIdx.x;
+  float s = 0.0f;
+  if (c < cols)
+    for (int64_t i = threadIdx.y; i < count; i += 8) s += part[(g * count + i) * row_stride + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+    out[g * cols + c] = s;
+  }
+}
+
+template <typename T>
+cudaError_t grad_launch(const ResidualNormGradArgs& a, int sm_count, cudaStream_t s) {
+  const GradChunks ck = grad_chunks(a, sm_count);
+  float2* stat = static_cast<float2*>(a.ws);
+  float* part = reinterpret_cast<float*>(stat + (a.rows + 15) / 16 * 16);
+  const int64_t v = (a.cols + 7) / 8;
+  const int tpr = v <= 32 ? 32 : v <= 64 ? 64 : v <= 128 ? 128 : 256;
+  const int rpc = tpr == 32 ? 4 : 1;
+  grad_stat_kernel<T><<<(unsigned)((a.rows + rpc - 1) / rpc), dim3(tpr, rpc), 0, s>>>(a, stat);
+  const unsigned col_tiles = (unsigned)((a.cols + kGradCols - 1) / kGradCols);
+  grad_cols_kernel<T><<<dim3((unsigned)ck.chunks, col_tiles), dim3(32, kLanes), 0, s>>>(a, ck, stat,
+                                                                                        part);
+  const unsigned sums = (unsigned)((a.cols + 31) / 32);
+  if (a.dw_pre)
+    grad_sum_kernel<<<dim3(1, sums), dim3(32, 8), 0, s>>>(part, 3 * a.cols, ck.chunks, a.cols, a.dw_pre);
+  if (a.dw_post)
+    grad_sum_kernel<<<dim3(1, sums), dim3(32, 8), 0, s>>>(part + a.cols, 3 * a.cols, ck.chunks, a.cols,
+                                                          a.dw_post);
+  if (a.dgate && !ck.whole)
+    grad_sum_kernel<<<dim3((unsigned)ck.gates, sums), dim3(32, 8), 0, s>>>(
+        part + 2 * a.cols, 3 * a.cols, ck.per_gate, a.cols, a.dgate);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_residual_norm(int type, int h_fmt, const ResidualNormArgs& a, int sm_count,
+                                 cudaStream_t s) {
+  if (type == B2G_F32) return norm_fmt<float>(h_fmt, a, sm_count, s);
+  if (type == B2G_BF16) return norm_fmt<__nv_bfloat16>(h_fmt, a, sm_count, s);
+  return norm_fmt<__half>(h_fmt, a, sm_count, s);
+}
+
+size_t norm_grad_ws_bytes(int type, const ResidualNormGradArgs& a, int sm_count) {
+  (void)type;
+  const GradChunks ck = grad_chunks(a, sm_count);
+  return (size_t)(a.rows + 15) / 16 * 16 * sizeof(float2) +
+         (size_t)ck.chunks * 3 * (size_t)a.cols * sizeof(float);
+}
+
+cudaError_t launch_residual_norm_grad(int type, const ResidualNormGradArgs& a, int sm_count,
+                                      cudaStream_t s) {
+  if (type == B2G_F32) return grad_launch<float>(a, sm_count, s);
+  if (type == B2G_BF16) return grad_launch<__nv_bfloat16>(a, sm_count, s);
+  return grad_launch<__half>(a, sm_count, s);
+}
+
+}  // namespace b2g
