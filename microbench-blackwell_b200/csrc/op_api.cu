@@ -317,9 +317,10 @@ b2g_status b2g_linear(b2g_handle* h, const b2g_linear_desc* d, void* stream) {
   if (d->type == B2G_F32)
     return fail(h, B2G_ERR_UNSUPPORTED, "b2g_linear: x must be bf16 or fp16");
   if (!type_ok(d->type)) return fail(h, B2G_ERR_INVALID, "b2g_linear: type %d", d->type);
-  if (d->T < 0 || d->N < 0 || d->K < 1 || d->T > kFewMaxTokens || d->N >= kMaxExtent ||
-      d->K >= kMaxExtent)
-    return fail(h, B2G_ERR_INVALID, "b2g_linear: T, N or K out of range (T up to %d)", kFewMaxTokens);
+  if (d->T < 0 || d->N < 0 || d->K < 1 || d->T > kFewMaxTokens || d->N > kFewMaxExtent ||
+      d->K > kFewMaxExtent)
+    return fail(h, B2G_ERR_INVALID, "b2g_linear: T, N or K out of range (T up to %d, N and K to %d)",
+                kFewMaxTokens, kFewMaxExtent);
   if (d->T == 0 || d->N == 0) return B2G_OK;
   if (!matrix_ok(d->x, d->type, d->K, d->ld_x) || !matrix_ok(d->out, d->type, d->N, d->ld_out) ||
       !d->w || !d->sfw || !aligned(d->w, 16) || !aligned(d->sfw, 2))

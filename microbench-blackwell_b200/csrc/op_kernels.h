@@ -72,6 +72,7 @@ cudaError_t launch_residual_norm_grad(int type, const ResidualNormGradArgs& a, i
 
 // Few-token product with microscaled weights (few_linear.cu).
 constexpr int kFewMaxTokens = 65536;
+constexpr int kFewMaxExtent = 1 << 24;  // N and K: indexes within a matrix's edge are 32 bits
 struct FewLinearArgs {
   int64_t T, N, K, kp;
   const void* x;
