@@ -96,6 +96,43 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
   }
 }
 
+// Two fp32 in one register pair: one instruction for both.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+// the same as four pairs
+template <typename T>
+__device__ __forceinline__ void unpack4x2(const Raw8<T>& r, float2 (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = make_float2(__uint_as_float(r.w[0].x), __uint_as_float(r.w[0].y));
+    v[1] = make_float2(__uint_as_float(r.w[0].z), __uint_as_float(r.w[0].w));
+    v[2] = make_float2(__uint_as_float(r.w[1].x), __uint_as_float(r.w[1].y));
+    v[3] = make_float2(__uint_as_float(r.w[1].z), __uint_as_float(r.w[1].w));
+  } else {
+    v[0] = pair_f32<T>(r.w[0].x);
+    v[1] = pair_f32<T>(r.w[0].y);
+    v[2] = pair_f32<T>(r.w[0].z);
+    v[3] = pair_f32<T>(r.w[0].w);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -125,6 +162,12 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool ve
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < n) p[i] = from_f32<T>(v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4x2(T* p, const float2 (&v)[4], bool vec) {
+  const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+  store8(p, f, 8, vec);
 }
 
 // ---------------------------------------------------------------- microscaled codes

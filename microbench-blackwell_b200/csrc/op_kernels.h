@@ -64,6 +64,7 @@ struct ResidualNormGradArgs {
   float *dgate, *dw_post, *dw_pre;
   float alpha, beta;
   int vec;
+  int dgate_vec;  // dgate starts on 16 bytes
   void* ws;  // norm_grad_ws_bytes() bytes
 };
 size_t norm_grad_ws_bytes(int type, const ResidualNormGradArgs& a, int sm_count);
