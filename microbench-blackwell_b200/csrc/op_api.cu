@@ -302,6 +302,7 @@ b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_norm_gra
           vec(d->dy, d->ld_dy) && vec(d->gate, d->cols) && aligned(d->w_post, 16) &&
           aligned(d->w_pre, 16);
   a.dgate_vec = aligned(d->dgate, 16);
+  a.err = h->d_err;
   const b2g_status st = grow(h, norm_grad_ws_bytes(type, a, h->sm_count), 0, s);
   if (st != B2G_OK) return st;
   a.ws = h->op_ws;

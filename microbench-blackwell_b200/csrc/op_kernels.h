@@ -65,6 +65,7 @@ struct ResidualNormGradArgs {
   float alpha, beta;
   int vec;
   int dgate_vec;  // dgate starts on 16 bytes
+  uint32_t* err;  // the handle's error word
   void* ws;  // norm_grad_ws_bytes() bytes
 };
 size_t norm_grad_ws_bytes(int type, const ResidualNormGradArgs& a, int sm_count);

@@ -511,9 +511,9 @@ GradRows grad_rows(int type, const ResidualNormGradArgs& a, int sm_count) {
   const int64_t v = a.cols / 8;
   if (!a.vec || a.cols % 8 || v > 1024) return p;
   const int es = type == B2G_F32 ? 4 : 2;
-  p.nv = v > 128 ? 2 : 1;
-  p.max_threads = v > 512 ? 512 : v > 128 ? 256 : 128;
+  p.nv = v > 512 ? 2 : 1;
   const int threads = ((int)((v + p.nv - 1) / p.nv) + 31) / 32 * 32;
+  p.max_threads = threads > 256 ? 512 : threads > 128 ? 256 : 128;
   p.gate_rows = a.gate && a.rows_per_gate < 8 && a.rows_per_gate < a.rows;
   const size_t stage = (size_t)p.max_threads * p.nv * (p.gate_rows ? 5 : 4) * 8 * es;
   // CTAs on an SM: by registers (128 a thread) and shared memory
@@ -545,9 +545,10 @@ cudaError_t grad_rows_main(const ResidualNormGradArgs& a, const GradRows& p, flo
 template <typename T, bool ALL, bool FEW>
 cudaError_t grad_rows_shape(const ResidualNormGradArgs& a, const GradRows& p, float* part, float* slots,
                             cudaStream_t s) {
+  if (p.nv == 2) return grad_rows_main<T, 2, 512, ALL, FEW>(a, p, part, slots, s);
   if (p.max_threads == 128) return grad_rows_main<T, 1, 128, ALL, FEW>(a, p, part, slots, s);
-  if (p.max_threads == 256) return grad_rows_main<T, 2, 256, ALL, FEW>(a, p, part, slots, s);
-  return grad_rows_main<T, 2, 512, ALL, FEW>(a, p, part, slots, s);
+  if (p.max_threads == 256) return grad_rows_main<T, 1, 256, ALL, FEW>(a, p, part, slots, s);
+  return grad_rows_main<T, 1, 512, ALL, FEW>(a, p, part, slots, s);
 }
 
 template <typename T>
