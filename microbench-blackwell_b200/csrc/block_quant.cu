@@ -24,58 +24,104 @@ __device__ __forceinline__ uint2 load_rand8(const uint8_t* p, int n, bool vec) {
   return make_uint2(w[0], w[1]);
 }
 
-// Codes and scale of eight elements held by one thread; the threads of a block (2 for
-// 16 elements, 4 for 32) are neighbours and share the largest magnitude.
-template <int FMT, int QM, bool SR>
-__device__ __forceinline__ void encode_row8(float (&x)[8], float scale, uint2 rnd,
-                                            uint8_t* codes, uint8_t* sf, bool write) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = __fmul_rn(x[i], scale);
-    amax = max_nan(amax, fabsf(x[i]));
-  }
-  amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-  if constexpr (bf_block(FMT) == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-  const BlockScale s = block_scale<FMT>(amax);
-  uint32_t w[2];
-  encode8<FMT, QM, SR>(x, s, rnd, w);
-  if (!write) return;
-  if constexpr (FMT == BF_MXF8)
-    *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
-  else
-    *reinterpret_cast<uint32_t*>(codes) = w[0];
-  if ((threadIdx.x & (bf_block(FMT) / 8 - 1)) == 0) *sf = (uint8_t)s.byte;
+// A thread's 16 elements of a row: a block of NVFP4, half of an MX block (its neighbour has
+// the other half).
+template <typename T>
+struct Raw16 {
+  Raw8<T> h[2];
+};
+
+// 16 random bytes, zeros from the n-th on
+struct Rand16 {
+  uint2 h[2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw16<T> load16(const T* p, int n, bool vec) {
+  Raw16<T> r;
+  r.h[0] = load8(p, n < 8 ? n : 8, vec);
+  r.h[1] = load8(p + 8, n < 8 ? 0 : n - 8, vec);
+  return r;
 }
 
-// Rows only: eight elements per thread.  blockDim.x threads along a row, blockDim.y rows.
-template <typename T, int FMT, int QM, bool SR>
+__device__ __forceinline__ Rand16 load_rand16(const uint8_t* p, int n, bool vec) {
+  Rand16 r;
+  r.h[0] = load_rand8(p, n < 8 ? n : 8, vec);
+  r.h[1] = load_rand8(p + 8, n < 8 ? 0 : n - 8, vec);
+  return r;
+}
+
+template <int FMT, int QM, bool SR>
+__device__ __forceinline__ void store_row16(const float2 (&x)[2][4], const BlockScale& s, float fold,
+                                            const Rand16& rnd, uint8_t* codes, uint8_t* sf) {
+  uint32_t lo[2], hi[2];
+  encode8<FMT, QM, SR>(x[0], s, fold, rnd.h[0], lo);
+  encode8<FMT, QM, SR>(x[1], s, fold, rnd.h[1], hi);
+  if constexpr (FMT == BF_MXF8)
+    *reinterpret_cast<uint4*>(codes) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
+  else
+    *reinterpret_cast<uint2*>(codes) = make_uint2(lo[0], hi[0]);
+  if (bf_block(FMT) == 16 || (threadIdx.x & 1) == 0) *sf = (uint8_t)s.byte;
+}
+
+// Codes and scale of 16 elements of a row.  All lanes of a warp take part.
+template <typename T, int FMT, int QM, bool SR, bool PRE>
+__device__ __forceinline__ void encode_row16(const Raw16<T>& raw, float scale, const Rand16& rnd,
+                                             uint8_t* codes, uint8_t* sf, bool write) {
+  float2 x[2][4];
+  float amax;
+  if constexpr (PRE) {
+    amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      unpack4x2(raw.h[k], x[k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[k][i] = mul2(x[k][i], both(scale));
+        amax = max_nan(amax, max_nan(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+      }
+    }
+  } else {
+    const uint4 a = raw.h[0].w[0], b = raw.h[1].w[0];
+    const uint32_t m = absmax_pair<T>(
+        absmax_pair<T>(absmax_pair<T>(a.x, a.y), absmax_pair<T>(a.z, a.w)),
+        absmax_pair<T>(absmax_pair<T>(b.x, b.y), absmax_pair<T>(b.z, b.w)));
+    const float2 f = pair_f32<T>(m);
+    amax = max_nan(f.x, f.y) * scale;
+    unpack4x2(raw.h[0], x[0]);
+    unpack4x2(raw.h[1], x[1]);
+  }
+  if constexpr (bf_block(FMT) == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+  const BlockScale s = block_scale<FMT, QM>(amax);
+  if (write) store_row16<FMT, QM, SR>(x, s, PRE ? 1.0f : scale, rnd, codes, sf);
+}
+
+// Rows only: 16 elements per thread.  blockDim.x threads along a row, blockDim.y rows.
+template <typename T, int FMT, int QM, bool SR, bool PRE>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const BlockQuantArgs a) {
   constexpr int bits = bf_bits(FMT), blk = bf_block(FMT);
-  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 16;
   const bool in_row = c < a.kp;
-  const int n = c >= a.cols ? 0 : (int)(a.cols - c < 8 ? a.cols - c : 8);
+  const int n = c >= a.cols ? 0 : (int)(a.cols - c < 16 ? a.cols - c : 16);
   const int64_t step = (int64_t)gridDim.y * blockDim.y;
-  // two rows at a time: both loads are in flight before the first is used
+  // two rows at a time: the loads of both are in flight before the first is used
   for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; __any_sync(0xFFFFFFFFu, r < a.rows);
        r += 2 * step) {
     const bool ok0 = in_row && r < a.rows, ok1 = in_row && r + step < a.rows;
     const T* p = static_cast<const T*>(a.in) + r * a.ld_in + c;
-    const Raw8<T> raw0 = load8(p, ok0 ? n : 0, a.in_vec);
-    const Raw8<T> raw1 = load8(p + step * a.ld_in, ok1 ? n : 0, a.in_vec);
-    uint2 rnd0 = make_uint2(0, 0), rnd1 = rnd0;
+    const Raw16<T> raw0 = load16(p, ok0 ? n : 0, a.in_vec);
+    const Raw16<T> raw1 = load16(p + step * a.ld_in, ok1 ? n : 0, a.in_vec);
+    Rand16 rnd0, rnd1;
     if constexpr (SR) {
       const uint8_t* q = a.rand + r * a.ld_rand + c;
-      rnd0 = load_rand8(q, ok0 ? n : 0, a.rand_vec);
-      rnd1 = load_rand8(q + step * a.ld_rand, ok1 ? n : 0, a.rand_vec);
+      rnd0 = load_rand16(q, ok0 ? n : 0, a.rand_vec);
+      rnd1 = load_rand16(q + step * a.ld_rand, ok1 ? n : 0, a.rand_vec);
     }
-    float x[8];
-    unpack8(raw0, x);
-    encode_row8<FMT, QM, SR>(x, a.scale, rnd0, a.codes + (r * a.kp + c) * bits / 8,
-                             a.sf + (r * a.kp + c) / blk, ok0);
-    unpack8(raw1, x);
-    encode_row8<FMT, QM, SR>(x, a.scale, rnd1, a.codes + ((r + step) * a.kp + c) * bits / 8,
-                             a.sf + ((r + step) * a.kp + c) / blk, ok1);
+    encode_row16<T, FMT, QM, SR, PRE>(raw0, a.scale, rnd0, a.codes + (r * a.kp + c) * bits / 8,
+                                      a.sf + (r * a.kp + c) / blk, ok0);
+    encode_row16<T, FMT, QM, SR, PRE>(raw1, a.scale, rnd1,
+                                      a.codes + ((r + step) * a.kp + c) * bits / 8,
+                                      a.sf + ((r + step) * a.kp + c) / blk, ok1);
   }
 }
 
@@ -88,90 +134,122 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const BlockQuantAr
 // column word then read different banks.
 constexpr int kTileRows = 128;
 
-template <typename T, int FMT, int QM, bool SR, bool ROWS>
+template <typename T, int FMT, int QM, bool SR, bool PRE, bool ROWS>
 __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantArgs a) {
   constexpr int bits = bf_bits(FMT), blk = bf_block(FMT);
   constexpr int kCols = 128 / (int)sizeof(T);    // columns of a tile
-  constexpr int kVec = kCols / 8;                // eights of a row
+  constexpr int kVec = kCols / 16;               // sixteens of a row
   constexpr int kPer = 4 / (int)sizeof(T);       // columns of a 32-bit word
+  constexpr int kRandWords = kCols / 4;          // words of a row of random bytes
   __shared__ __align__(16) uint32_t tile[kTileRows * 32];
-  __shared__ __align__(16) uint8_t rnd_tile[SR ? kTileRows * kCols : 16];
+  __shared__ __align__(16) uint32_t rnd_tile[SR ? kTileRows * kRandWords : 4];
   const int tid = threadIdx.x;
   const unsigned col_tiles = (unsigned)((a.kp + kCols - 1) / kCols);
   const int64_t r0 = (int64_t)(blockIdx.x / col_tiles) * kTileRows;
   const int64_t c0 = (int64_t)(blockIdx.x % col_tiles) * kCols;
 
+  constexpr int kItems = kTileRows * kVec / kThreads;
+  Raw16<T> raw[kItems];
 #pragma unroll
-  for (int i = 0; i < kTileRows * kVec / kThreads; ++i) {
+  for (int i = 0; i < kItems; ++i) {
+    const int item = i * kThreads + tid;
+    const int64_t r = r0 + item / kVec, c = c0 + item % kVec * 16;
+    const int n = r >= a.rows || c >= a.cols ? 0 : (int)(a.cols - c < 16 ? a.cols - c : 16);
+    raw[i] = load16(static_cast<const T*>(a.in) + r * a.ld_in + c, n, a.in_vec);
+  }
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
     const int item = i * kThreads + tid, v = item % kVec, lr = item / kVec;
-    const int64_t r = r0 + lr, c = c0 + v * 8;
-    const int n = r >= a.rows || c >= a.cols ? 0 : (int)(a.cols - c < 8 ? a.cols - c : 8);
-    const Raw8<T> raw = load8(static_cast<const T*>(a.in) + r * a.ld_in + c, n, a.in_vec);
-    uint2 rnd = make_uint2(0, 0);
+    const int64_t r = r0 + lr, c = c0 + v * 16;
     const int g = (lr >> 4) & 7;
+    Rand16 rnd;
     if constexpr (SR) {
-      rnd = load_rand8(a.rand + r * a.ld_rand + c, n, a.rand_vec);
-      // 32-bit word q of a row lies at q ^ 2 g (fp32 tiles: half as many words)
-      uint32_t* q = reinterpret_cast<uint32_t*>(rnd_tile) + lr * (kCols / 4);
-      const int at = (2 * v) ^ ((2 * g) & (kCols / 4 - 1));
-      *reinterpret_cast<uint2*>(q + at) = rnd;
+      const int n = r >= a.rows || c >= a.cols ? 0 : (int)(a.cols - c < 16 ? a.cols - c : 16);
+      rnd = load_rand16(a.rand + r * a.ld_rand + c, n, a.rand_vec);
+      // pair p of 32-bit words of a row lies at p ^ g (fp32 tiles: half as many pairs)
+      uint2* q = reinterpret_cast<uint2*>(rnd_tile) + lr * (kRandWords / 2);
+      q[(2 * v) ^ (g & (kRandWords / 2 - 1))] = rnd.h[0];
+      q[(2 * v + 1) ^ (g & (kRandWords / 2 - 1))] = rnd.h[1];
     }
     uint4* row = reinterpret_cast<uint4*>(tile) + lr * 8;
     if constexpr (sizeof(T) == 4) {
-      row[(2 * v) ^ g] = raw.w[0];
-      row[(2 * v + 1) ^ g] = raw.w[1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) row[(4 * v + k) ^ g] = raw[i].h[k >> 1].w[k & 1];
     } else {
-      row[v ^ g] = raw.w[0];
+      row[(2 * v) ^ g] = raw[i].h[0].w[0];
+      row[(2 * v + 1) ^ g] = raw[i].h[1].w[0];
     }
-    if constexpr (ROWS) {
-      float x[8];
-      unpack8(raw, x);
-      encode_row8<FMT, QM, SR>(x, a.scale, rnd, a.codes + (r * a.kp + c) * bits / 8,
-                               a.sf + (r * a.kp + c) / blk, r < a.rows && c < a.kp);
-    }
+    if constexpr (ROWS)
+      encode_row16<T, FMT, QM, SR, PRE>(raw[i], a.scale, rnd, a.codes + (r * a.kp + c) * bits / 8,
+                                        a.sf + (r * a.kp + c) / blk, r < a.rows && c < a.kp);
   }
   __syncthreads();
 
   const int g = tid & 7, w = tid >> 3;  // 16-row group, 32-bit word of the row
-  uint32_t raw[16];
+  uint32_t word[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    raw[i] = tile[(g * 16 + i) * 32 + ((((w >> 2) ^ g) << 2) | (w & 3))];
+    word[i] = tile[(g * 16 + i) * 32 + ((((w >> 2) ^ g) << 2) | (w & 3))];
   const int64_t r = r0 + g * 16;
+  // the word's columns side by side: largest magnitudes of both at a time
+  float2 amax;
+  float2 x[16];
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (PRE) {
+      amax = both(0.0f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[i] = mul2(pair_f32<T>(word[i]), both(a.scale));
+        amax = make_float2(max_nan(amax.x, fabsf(x[i].x)), max_nan(amax.y, fabsf(x[i].y)));
+      }
+    } else {
+      uint32_t m = absmax_pair<T>(word[0], word[1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) m = absmax_pair<T>(m, word[i]);
+      amax = mul2(pair_f32<T>(m), both(a.scale));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = pair_f32<T>(word[i]);
+    }
+  } else {
+    amax = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = make_float2(__fmul_rn(__uint_as_float(word[i]), a.scale), 0.0f);
+      amax.x = max_nan(amax.x, fabsf(x[i].x));
+    }
+  }
+  if constexpr (blk == 32) {
+    amax.x = max_nan(amax.x, __shfl_xor_sync(0xFFFFFFFFu, amax.x, 1));
+    if constexpr (kPer == 2) amax.y = max_nan(amax.y, __shfl_xor_sync(0xFFFFFFFFu, amax.y, 1));
+  }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int64_t c = c0 + w * kPer + j;
-    float x[2][8];
-    float amax = 0.0f;
+    const BlockScale s = block_scale<FMT, QM>(j ? amax.y : amax.x);
+    float2 y[2][4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float f;
-      if constexpr (sizeof(T) == 4) {
-        f = __uint_as_float(raw[i]);
-      } else {
-        const float2 p = pair_f32<T>(raw[i]);
-        f = j ? p.y : p.x;
-      }
-      f = __fmul_rn(f, a.scale);
-      x[i >> 3][i & 7] = f;
-      amax = max_nan(amax, fabsf(f));
-    }
-    if constexpr (blk == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
-    const BlockScale s = block_scale<FMT>(amax);
+    for (int i = 0; i < 16; i += 2)
+      y[i >> 3][(i & 7) >> 1] = j ? make_float2(x[i].y, x[i + 1].y) : make_float2(x[i].x, x[i + 1].x);
     uint2 rnd[2] = {make_uint2(0, 0), make_uint2(0, 0)};
     if constexpr (SR) {
-      uint32_t b[4] = {0u, 0u, 0u, 0u};
-      const int byte = w * kPer + j;
-      const int at = (((byte >> 2) ^ ((2 * g) & (kCols / 4 - 1))) << 2) | (byte & 3);
+      // byte w * kPer + j of each of the 16 rows, gathered into four words
+      const int byte = w * kPer + j, pair = byte >> 3;
+      const int at = ((pair ^ (g & (kRandWords / 2 - 1))) << 1) | ((byte >> 2) & 1);
+      uint32_t b[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        b[i >> 2] |= (uint32_t)rnd_tile[(g * 16 + i) * kCols + at] << (8 * (i & 3));
+      for (int k = 0; k < 4; ++k) {
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = rnd_tile[(g * 16 + 4 * k + i) * kRandWords + at];
+        const uint32_t sel = (byte & 3) | (((byte & 3) + 4) << 4);
+        b[k] = __byte_perm(__byte_perm(q[0], q[1], sel), __byte_perm(q[2], q[3], sel), 0x5410);
+      }
       rnd[0] = make_uint2(b[0], b[1]);
       rnd[1] = make_uint2(b[2], b[3]);
     }
     uint32_t lo[2], hi[2];
-    encode8<FMT, QM, SR>(x[0], s, rnd[0], lo);
-    encode8<FMT, QM, SR>(x[1], s, rnd[1], hi);
+    encode8<FMT, QM, SR>(y[0], s, PRE ? 1.0f : a.scale, rnd[0], lo);
+    encode8<FMT, QM, SR>(y[1], s, PRE ? 1.0f : a.scale, rnd[1], hi);
     if (c < a.cols && r < a.tp) {
       uint8_t* dst = a.codes_t + (c * a.tp + r) * bits / 8;
       if constexpr (FMT == BF_MXF8)
@@ -183,51 +261,61 @@ __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantAr
   }
 }
 
-// Read-back: eight codes per thread.
+// Read-back: eight codes per thread, of four rows at a time so that their loads are in
+// flight together.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(const BlockDequantArgs a) {
-  constexpr int bits = bf_bits(FMT), blk = bf_block(FMT);
+  constexpr int bits = bf_bits(FMT), blk = bf_block(FMT), kRows = 4;
   const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
   if (c >= a.cols) return;
   const int n = (int)(a.cols - c < 8 ? a.cols - c : 8);
-  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < a.rows;
-       r += (int64_t)gridDim.y * blockDim.y) {
-    const int64_t e = r * a.kp + c;
-    const uint32_t sb = __ldg(a.sf + e / blk);
-    float s;
-    if constexpr (FMT == BF_NVFP4)
-      s = e4m3_pair(sb).x;
-    else
-      s = e8m0_value(sb);
-    float v[8];
-    if constexpr (FMT == BF_MXF8) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(a.codes + e));
+  const int64_t step = (int64_t)gridDim.y * blockDim.y;
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows * step) {
+    uint2 w[kRows];
+    uint32_t sb[kRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 p = e4m3_pair((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
-        v[2 * i] = p.x;
-        v[2 * i + 1] = p.y;
-      }
-    } else {
-      const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(a.codes + e * bits / 8));
-      uint32_t h[4];
-      e2m1x8_pairs(w, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-        v[2 * i] = p.x;
-        v[2 * i + 1] = p.y;
-      }
+    for (int k = 0; k < kRows; ++k) {
+      const int64_t r = r0 + k * step, e = (r < a.rows ? r : r0) * a.kp + c;
+      if constexpr (FMT == BF_MXF8)
+        w[k] = __ldg(reinterpret_cast<const uint2*>(a.codes + e));
+      else
+        w[k].x = __ldg(reinterpret_cast<const uint32_t*>(a.codes + e * bits / 8));
+      sb[k] = __ldg(a.sf + e / blk);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], s), a.scale);
-    store8(static_cast<T*>(a.out) + r * a.ld_out + c, v, n, a.out_vec);
+    for (int k = 0; k < kRows; ++k) {
+      const int64_t r = r0 + k * step;
+      if (r >= a.rows) break;
+      float s;
+      if constexpr (FMT == BF_NVFP4)
+        s = e4m3_pair(sb[k]).x;
+      else
+        s = e8m0_value(sb[k]);
+      float2 v[4];
+      if constexpr (FMT == BF_MXF8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = e4m3_pair((i < 2 ? w[k].x : w[k].y) >> (16 * (i & 1)));
+      } else {
+        uint32_t h[4];
+        e2m1x8_pairs(w[k].x, h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      }
+      // code * s is exact
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], both(s));
+      if (a.scale != 1.0f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], both(a.scale));
+      const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+      store8(static_cast<T*>(a.out) + r * a.ld_out + c, f, n, a.out_vec);
+    }
   }
 }
 
-// blockDim.x threads of eight elements along a row of `cols`, the rest along the rows
-void row_shape(int64_t rows, int64_t cols, dim3* grid, dim3* block) {
-  const int64_t v = (cols + 7) / 8;
+// blockDim.x threads of `per` elements along a row of `cols`, the rest along the rows
+void row_shape(int64_t rows, int64_t cols, int per, dim3* grid, dim3* block) {
+  const int64_t v = (cols + per - 1) / per;
   int bx = 4;
   while (bx < kThreads && bx < v) bx *= 2;
   const int by = kThreads / bx;
@@ -237,44 +325,50 @@ void row_shape(int64_t rows, int64_t cols, dim3* grid, dim3* block) {
   *grid = dim3((unsigned)gx, (unsigned)(gy < 65535 ? gy : 65535));
 }
 
-template <typename T, int FMT, int QM, bool SR>
+template <typename T, int FMT, int QM, bool SR, bool PRE>
 cudaError_t quant_launch(const BlockQuantArgs& a, cudaStream_t s) {
   if (!a.codes_t) {
     dim3 grid, block;
-    row_shape((a.rows + 1) / 2, a.kp, &grid, &block);
-    quant_rows_kernel<T, FMT, QM, SR><<<grid, block, 0, s>>>(a);
+    row_shape((a.rows + 1) / 2, a.kp, 16, &grid, &block);
+    quant_rows_kernel<T, FMT, QM, SR, PRE><<<grid, block, 0, s>>>(a);
     return cudaGetLastError();
   }
   constexpr int kCols = 128 / (int)sizeof(T);
   const int64_t tiles = ((a.tp + kTileRows - 1) / kTileRows) * ((a.kp + kCols - 1) / kCols);
   if (tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const unsigned grid = (unsigned)tiles;
   if (a.codes)
-    quant_both_kernel<T, FMT, QM, SR, true><<<grid, kThreads, 0, s>>>(a);
+    quant_both_kernel<T, FMT, QM, SR, PRE, true><<<(unsigned)tiles, kThreads, 0, s>>>(a);
   else
-    quant_both_kernel<T, FMT, QM, SR, false><<<grid, kThreads, 0, s>>>(a);
+    quant_both_kernel<T, FMT, QM, SR, PRE, false><<<(unsigned)tiles, kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, int FMT, int QM>
+template <typename T, int FMT, int QM, bool PRE>
 cudaError_t quant_sr(const BlockQuantArgs& a, cudaStream_t s) {
-  return a.rand ? quant_launch<T, FMT, QM, true>(a, s) : quant_launch<T, FMT, QM, false>(a, s);
+  return a.rand ? quant_launch<T, FMT, QM, true, PRE>(a, s)
+                : quant_launch<T, FMT, QM, false, PRE>(a, s);
 }
 
+// PRE: each element is multiplied by `scale` first.  16-bit inputs with a power of two need
+// not: it goes into the reciprocal of the block's scale.
 template <typename T>
 cudaError_t quant_fmt(int fmt, bool pow2, const BlockQuantArgs& a, cudaStream_t s) {
-  if (fmt == BF_MXF8) return quant_sr<T, BF_MXF8, Q_EXACT>(a, s);
-  if (fmt == BF_MXF4) return quant_sr<T, BF_MXF4, Q_EXACT>(a, s);
-  // the short quotient holds for inputs of at most 11 significant bits
-  if constexpr (sizeof(T) == 2)
-    if (pow2) return quant_sr<T, BF_NVFP4, Q_SNAP>(a, s);
-  return quant_sr<T, BF_NVFP4, Q_DIVIDE>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (pow2) {
+      if (fmt == BF_MXF8) return quant_sr<T, BF_MXF8, Q_EXACT, false>(a, s);
+      if (fmt == BF_MXF4) return quant_sr<T, BF_MXF4, Q_EXACT, false>(a, s);
+      return quant_sr<T, BF_NVFP4, Q_SNAP, false>(a, s);
+    }
+  }
+  if (fmt == BF_MXF8) return quant_sr<T, BF_MXF8, Q_EXACT, true>(a, s);
+  if (fmt == BF_MXF4) return quant_sr<T, BF_MXF4, Q_EXACT, true>(a, s);
+  return quant_sr<T, BF_NVFP4, Q_DIVIDE, true>(a, s);
 }
 
 template <typename T>
 cudaError_t dequant_fmt(int fmt, const BlockDequantArgs& a, cudaStream_t s) {
   dim3 grid, block;
-  row_shape(a.rows, a.cols, &grid, &block);
+  row_shape((a.rows + 3) / 4, a.cols, 8, &grid, &block);
   if (fmt == BF_MXF8)
     dequant_kernel<T, BF_MXF8><<<grid, block, 0, s>>>(a);
   else if (fmt == BF_MXF4)

@@ -115,6 +115,15 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
 
 // the same as four pairs
@@ -195,7 +204,7 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 }
 
 // eight e2m1 codes, element i in bits [4i, 4i + 4)
-__device__ __forceinline__ uint32_t e2m1x8(const float (&x)[8]) {
+__device__ __forceinline__ uint32_t e2m1x8(const float2 (&x)[4]) {
   uint32_t r;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -204,7 +213,8 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&x)[8]) {
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(r)
-      : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+      : "f"(x[0].x), "f"(x[0].y), "f"(x[1].x), "f"(x[1].y), "f"(x[2].x), "f"(x[2].y),
+        "f"(x[3].x), "f"(x[3].y));
   return r;
 }
 
@@ -232,21 +242,52 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
   return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7FFFFFFFu : byte << 23);
 }
 
-// The scale of a block from its largest magnitude: the stored byte, its value and
-// the reciprocal of the value (0 where all codes shall be 0).
+// Largest magnitudes of the halves of two words of 16-bit elements, NaN if one is.
+template <typename T>
+__device__ __forceinline__ uint32_t absmax_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (__is_same(T, __half))
+    asm("{\n\t.reg .b32 x, y;\n\tabs.f16x2 x, %1;\n\tabs.f16x2 y, %2;\n\t"
+        "max.NaN.f16x2 %0, x, y;\n\t}"
+        : "=r"(r)
+        : "r"(a), "r"(b));
+  else
+    asm("{\n\t.reg .b32 x, y;\n\tabs.bf16x2 x, %1;\n\tabs.bf16x2 y, %2;\n\t"
+        "max.NaN.bf16x2 %0, x, y;\n\t}"
+        : "=r"(r)
+        : "r"(a), "r"(b));
+  return r;
+}
+
+// How x / s is formed.  MX scales are powers of two: x * (1 / s) is exact.  NVFP4:
+//   Q_DIVIDE  x / s rounded to fp32, right for any x;
+//   Q_SNAP    for x with at most 11 significant bits (16-bit inputs times a power of
+//             two).  The boundaries of e2m1 have at most 3 bits and s has 4, so x / s
+//             either lies on a boundary or at least 2^-13 beside it.  fma(x, 1/s, 48)
+//             - 48 rounds the quotient to a multiple of 2^-18: a quotient on a boundary
+//             comes out on it and no other crosses one, for two instructions (two
+//             elements each) where the division takes about ten.  In the same way amax / 6
+//             comes from a product rounded to 16 bits: the boundaries of e4m3 have 5.
+enum QuotientMode : int { Q_EXACT = 0, Q_DIVIDE = 1, Q_SNAP = 2 };
+
+// The scale of a block from its largest magnitude: the stored byte, its value and the
+// reciprocal of the value (0 where all codes shall be 0), rounded up.
 struct BlockScale {
   uint32_t byte;
   float value, inv;
 };
 
-template <int FMT>
+template <int FMT, int QM>
 __device__ __forceinline__ BlockScale block_scale(float amax) {
   BlockScale s;
   const bool finite = amax < __uint_as_float(0x7F800000u);  // false for NaN too
   if constexpr (FMT == BF_NVFP4) {
-    s.byte = e4m3x2(amax / 6.0f, 0.0f) & 0xFFu;
+    const float sixth =
+        QM == Q_SNAP ? __uint_as_float((__float_as_uint(amax * (1.0f / 6.0f)) + 0x80u) & ~0xFFu)
+                     : amax / 6.0f;
+    s.byte = e4m3x2(sixth, 0.0f) & 0xFFu;
     s.value = e4m3_pair(s.byte).x;
-    s.inv = s.byte ? __frcp_rn(s.value) : 0.0f;
+    s.inv = s.byte ? __frcp_ru(s.value) : 0.0f;
     if (!finite) s = {0x7Fu, 0.0f, 0.0f};
   } else {
     constexpr int emax = FMT == BF_MXF8 ? 8 : 2;
@@ -260,65 +301,61 @@ __device__ __forceinline__ BlockScale block_scale(float amax) {
   return s;
 }
 
-// How x / s is formed.  MX scales are powers of two: x * (1 / s) is exact.  NVFP4:
-//   Q_DIVIDE  x / s rounded to fp32, right for any x;
-//   Q_SNAP    for x with at most 11 significant bits (16-bit inputs times a power of
-//             two).  The boundaries of e2m1 have at most 3 bits and s has 4, so x / s
-//             either lies on a boundary or at least 2^-13 beside it.  fma(x, 1/s, 48)
-//             - 48 rounds the quotient to a multiple of 2^-18: a quotient on a boundary
-//             comes out on it and no other crosses one, for two instructions where the
-//             division takes about ten.
-enum QuotientMode : int { Q_EXACT = 0, Q_DIVIDE = 1, Q_SNAP = 2 };
-
+// Stochastic rounding with a given byte r: |x / s| in steps of the element format goes up
+// when its fraction and (r + 1/2) / 256 together reach the next step.  |x / s| is scaled so
+// that the format's lowest binade becomes the lowest normal one of fp32: the bits of the
+// result then are the magnitude code with the fraction below it, subnormal codes included,
+// and (r + 1/2) / 256 of a step is added to them as an integer.  Q_SNAP: a fraction that
+// with r reaches the step exactly must not come out below; 1 / s and the product are
+// rounded up, and no other quotient lies that near (the thresholds have 12 bits).
 template <int FMT, int QM>
-__device__ __forceinline__ float quotient(float x, const BlockScale& s) {
-  if constexpr (QM == Q_DIVIDE) return s.inv != 0.0f ? x / s.value : 0.0f;
-  if constexpr (QM == Q_SNAP) return __fadd_rn(__fmaf_rn(x, s.inv, 48.0f), -48.0f);
-  return __fmul_rn(x, s.inv);
+__device__ __forceinline__ float round_stochastic(float x, const BlockScale& s, float mult,
+                                                  uint32_t word, int byte) {
+  constexpr float down = FMT == BF_MXF8 ? 0x1p-120f : 0x1p-126f;
+  constexpr float up = FMT == BF_MXF8 ? 0x1p120f : 0x1p126f;
+  constexpr int frac = FMT == BF_MXF8 ? 20 : 22;  // bits below the code
+  uint32_t bits;
+  if constexpr (QM == Q_DIVIDE)
+    bits = __float_as_uint(s.inv != 0.0f ? fabsf(x / s.value) * down : 0.0f);
+  else
+    bits = __float_as_uint(__fmul_ru(fabsf(x), mult));
+  const int at = frac - 8 - 8 * byte;  // where the byte belongs, from where it is
+  const uint32_t r = (at >= 0 ? word << at : word >> -at) & (0xFFu << (frac - 8));
+  bits = (bits + r + (1u << (frac - 9))) & (0xFFFFFFFFu << frac);
+  return __uint_as_float(bits | (__float_as_uint(x) & 0x80000000u)) * up;
 }
 
-// Stochastic rounding with a given byte r: |q| in steps of the element format goes up
-// when its fraction and (r + 1/2) / 256 together reach the next step.  Returns the
-// value on the format's grid.
-template <int FMT>
-__device__ __forceinline__ float round_stochastic(float q, uint32_t r) {
-  constexpr uint32_t low = FMT == BF_MXF8 ? 121u << 23 : 127u << 23;  // lowest binade
-  constexpr uint32_t mant = (FMT == BF_MXF8 ? 3u : 1u) << 23;
-  constexpr float top = FMT == BF_MXF8 ? 448.0f : 6.0f;
-  const float a = fabsf(q);
-  uint32_t e = __float_as_uint(a) & 0x7F800000u;
-  e = (e < low ? low : e) - mant;
-  const float step = __uint_as_float(e), inv = __uint_as_float((254u << 23) - e);
-  const float n = floorf(__fadd_rn(__fmul_rn(a, inv), __fmaf_rn((float)r, 0x1p-8f, 0x1p-9f)));
-  return copysignf(fminf(n * step, top), q);
-}
-
-// Q_SNAP's counterpart for stochastic rounding, whose thresholds have up to 12 bits:
-// x / s lies on a threshold or at least 2^-16 of itself beside it, so the quotient is
-// rounded to 20 significant bits.
-__device__ __forceinline__ float snap20(float q) {
-  return __uint_as_float((__float_as_uint(q) + 8u) & ~15u);
-}
-
-// Codes of eight elements of one block: 32 bits (e2m1) in w[0] or 64 (e4m3) in w[0..1].
-// rnd: eight random bytes, used when SR.
+// Codes of eight elements of one block (times `fold`, a power of two): 32 bits (e2m1) in
+// w[0] or 64 (e4m3) in w[0..1].  rnd: eight random bytes, used when SR.
 template <int FMT, int QM, bool SR>
-__device__ __forceinline__ void encode8(const float (&x)[8], const BlockScale& s, uint2 rnd,
-                                        uint32_t (&w)[2]) {
-  float q[8];
+__device__ __forceinline__ void encode8(const float2 (&x)[4], const BlockScale& s, float fold,
+                                        uint2 rnd, uint32_t (&w)[2]) {
+  float2 q[4];
+  const float mult = s.inv * fold;
+  if constexpr (SR) {
+    const float m = mult * (FMT == BF_MXF8 ? 0x1p-120f : 0x1p-126f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (SR) {
-      float t = QM == Q_DIVIDE ? quotient<FMT, Q_DIVIDE>(x[i], s) : __fmul_rn(x[i], s.inv);
-      if constexpr (QM == Q_SNAP) t = snap20(t);
-      q[i] = round_stochastic<FMT>(t, ((i < 4 ? rnd.x : rnd.y) >> (8 * (i & 3))) & 0xFFu);
-    } else {
-      q[i] = quotient<FMT, QM>(x[i], s);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = i < 2 ? rnd.x : rnd.y;
+      q[i].x = round_stochastic<FMT, QM>(x[i].x, s, m, word, 2 * (i & 1));
+      q[i].y = round_stochastic<FMT, QM>(x[i].y, s, m, word, 2 * (i & 1) + 1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (QM == Q_DIVIDE) {
+        q[i].x = s.inv != 0.0f ? x[i].x / s.value : 0.0f;
+        q[i].y = s.inv != 0.0f ? x[i].y / s.value : 0.0f;
+      } else if constexpr (QM == Q_SNAP) {
+        q[i] = add2(fma2(x[i], both(mult), both(48.0f)), both(-48.0f));
+      } else {
+        q[i] = mul2(x[i], both(mult));
+      }
     }
   }
   if constexpr (FMT == BF_MXF8) {
-    w[0] = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
-    w[1] = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
+    w[0] = e4m3x2(q[0].x, q[0].y) | (e4m3x2(q[1].x, q[1].y) << 16);
+    w[1] = e4m3x2(q[2].x, q[2].y) | (e4m3x2(q[3].x, q[3].y) << 16);
   } else {
     w[0] = e2m1x8(q);
     w[1] = 0u;

@@ -127,14 +127,17 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
     if (a.h) store8(static_cast<T*>(a.h) + row * a.ld_h + col[j], v[j], n[j], vec);
     if constexpr (HF >= 0) {
       constexpr int blk = bf_block(HF), bits = bf_bits(HF);
+      constexpr int mode = HF == BF_NVFP4 ? Q_DIVIDE : Q_EXACT;
       float amax = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[j][i]));
       amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
       if constexpr (blk == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
-      const BlockScale s = block_scale<HF>(amax);
+      const BlockScale s = block_scale<HF, mode>(amax);
+      const float2 x2[4] = {make_float2(v[j][0], v[j][1]), make_float2(v[j][2], v[j][3]),
+                            make_float2(v[j][4], v[j][5]), make_float2(v[j][6], v[j][7])};
       uint32_t q[2];
-      encode8<HF, HF == BF_NVFP4 ? Q_DIVIDE : Q_EXACT, false>(v[j], s, make_uint2(0, 0), q);
+      encode8<HF, mode, false>(x2, s, 1.0f, make_uint2(0, 0), q);
       if (col[j] < width) {
         const int64_t e = row * a.kp + col[j];
         if constexpr (HF == BF_MXF8)
