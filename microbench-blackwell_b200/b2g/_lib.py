@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libb2g.so")
@@ -143,6 +144,13 @@ class LinearDesc(C.Structure):
         ("alpha", C.c_float), ("reserved", C.c_int32)]
 
 
+# The same descriptors packed from their values in order, native sizes and alignment
+BLOCK_QUANT = struct.Struct("@ii3q6Qqfi").pack
+RESIDUAL_NORM = struct.Struct("@ii7q11Q3fi").pack
+RESIDUAL_NORM_GRAD = struct.Struct("@ii9q14Q2f").pack
+LINEAR = struct.Struct("@ii5q4Qfi").pack
+
+
 # (name, restype, argtypes) of every exported entry point of include/b2g.h
 _SIGS = [
     ("b2g_abi_version", C.c_int, []),
@@ -197,14 +205,14 @@ _SIGS = [
     ("b2g_sparse_meta_bytes", C.c_size_t, [C.c_int64, C.c_int64]),
     ("b2g_sparse_meta_prepare", C.c_int,
      [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
-    ("b2g_block_quantize", C.c_int, [C.c_void_p, C.POINTER(BlockQuantDesc), C.c_void_p]),
+    ("b2g_block_quantize", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("b2g_block_dequantize", C.c_int,
      [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p,
       C.c_int64, C.c_float, C.c_void_p]),
-    ("b2g_residual_norm", C.c_int, [C.c_void_p, C.POINTER(ResidualNormDesc), C.c_void_p]),
+    ("b2g_residual_norm", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("b2g_residual_norm_backward", C.c_int,
-     [C.c_void_p, C.POINTER(ResidualNormGradDesc), C.c_void_p]),
-    ("b2g_linear", C.c_int, [C.c_void_p, C.POINTER(LinearDesc), C.c_void_p]),
+     [C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("b2g_linear", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("b2g_trace_enable", C.c_int, [C.c_void_p, C.c_int]),
     ("b2g_trace_read", C.c_int, [C.c_void_p, C.POINTER(C.c_uint32), C.c_int]),
     ("b2g_encode_idesc", C.c_uint32, [C.c_int] * 7),

@@ -313,13 +313,15 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(const BlockDequantArg
   }
 }
 
-// blockDim.x threads of `per` elements along a row of `cols`, the rest along the rows
+// blockDim.x threads of `per` elements along a row of `cols`, the rest along the rows: whole
+// warps, and with more than 128 threads to a row as few idle ones as 32 allow
 void row_shape(int64_t rows, int64_t cols, int per, dim3* grid, dim3* block) {
   const int64_t v = (cols + per - 1) / per;
+  const int64_t gx = (v + kThreads - 1) / kThreads;
   int bx = 4;
-  while (bx < kThreads && bx < v) bx *= 2;
+  while (bx < v && bx < 128) bx *= 2;
+  if (v > 128) bx = (int)((v + gx - 1) / gx + 31) / 32 * 32;
   const int by = kThreads / bx;
-  const int64_t gx = (v + bx - 1) / bx;
   int64_t gy = (rows + by - 1) / by;
   *block = dim3(bx, by);
   *grid = dim3((unsigned)gx, (unsigned)(gy < 65535 ? gy : 65535));

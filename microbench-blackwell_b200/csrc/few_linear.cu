@@ -611,8 +611,8 @@ cudaError_t few_launch(const FewLinearArgs& a, const FewShape& sh, cudaStream_t 
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int smem = sh.x_bytes + kWarps * kAhead * Ring<FMT>::kSlot;
-  e = cudaFuncSetAttribute(few_linear_kernel<T, FMT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           smem);
+  static std::atomic<int> seen[16];
+  e = allow_smem(few_linear_kernel<T, FMT, NT>, smem, seen);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;

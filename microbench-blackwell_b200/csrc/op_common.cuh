@@ -6,7 +6,23 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace b2g {
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device.  The attribute
+// is set once for each kernel, device and size above the last (`seen`: one word per device,
+// the kernel's own).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[16]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 16 && seen[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 16) seen[dev].store(bytes, std::memory_order_relaxed);
+  return e;
+}
 
 // Eight consecutive elements of a row as they lie in memory: one 16-byte word for
 // 16-bit types, two for fp32.
@@ -319,10 +335,10 @@ __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s, 
     bits = __float_as_uint(s.inv != 0.0f ? fabsf(x / s.value) * down : 0.0f);
   else
     bits = __float_as_uint(__fmul_ru(fabsf(x), mult));
-  const int at = frac - 8 - 8 * byte;  // where the byte belongs, from where it is
-  const uint32_t r = (at >= 0 ? word << at : word >> -at) & (0xFFu << (frac - 8));
-  bits = (bits + r + (1u << (frac - 9))) & (0xFFFFFFFFu << frac);
-  return __uint_as_float(bits | (__float_as_uint(x) & 0x80000000u)) * up;
+  // 256 r + 128: the byte above a half, one permutation
+  const uint32_t r = __byte_perm(word, 0x80u, 0x5504u | (uint32_t)(byte << 4));
+  bits = (r * (1u << (frac - 16)) + bits) & (0xFFFFFFFFu << frac);
+  return __uint_as_float(bits) * __uint_as_float((__float_as_uint(x) & 0x80000000u) | __float_as_uint(up));
 }
 
 // Codes of eight elements of one block (times `fold`, a power of two): 32 bits (e2m1) in

@@ -538,8 +538,8 @@ GradRows grad_rows(int type, const ResidualNormGradArgs& a, int sm_count) {
 template <typename T, int NV, int MAXT, bool ALL, bool FEW>
 cudaError_t grad_rows_main(const ResidualNormGradArgs& a, const GradRows& p, float* part, float* slots,
                            cudaStream_t s) {
-  const cudaError_t e = cudaFuncSetAttribute(grad_rows_kernel<T, NV, MAXT, ALL, FEW>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  static std::atomic<int> seen[16];
+  const cudaError_t e = allow_smem(grad_rows_kernel<T, NV, MAXT, ALL, FEW>, (int)p.smem, seen);
   if (e != cudaSuccess) return e;
   grad_rows_kernel<T, NV, MAXT, ALL, FEW><<<p.ctas, p.threads, p.smem, s>>>(a, p, part, slots);
   return cudaGetLastError();

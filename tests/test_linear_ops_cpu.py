@@ -28,6 +28,18 @@ def test_structs_match_the_c_layout(tmp_path, struct, ctype):
         assert int(got[n]) == getattr(cls, n).offset, n
 
 
+@pytest.mark.parametrize("pack,ctype", [
+    (_lib.BLOCK_QUANT, "BlockQuantDesc"), (_lib.RESIDUAL_NORM, "ResidualNormDesc"),
+    (_lib.RESIDUAL_NORM_GRAD, "ResidualNormGradDesc"), (_lib.LINEAR, "LinearDesc")])
+def test_packed_descriptors_match_the_structs(pack, ctype):
+    cls = getattr(_lib, ctype)
+    values = [i + 1 for i in range(len(cls._fields_))]
+    data = pack(*values)
+    assert len(data) == C.sizeof(cls)
+    d = cls.from_buffer_copy(data)
+    assert [getattr(d, n) for n, _ in cls._fields_] == values
+
+
 def test_a_null_handle_or_descriptor_is_refused():
     lib = _lib.load()
     assert lib.b2g_block_quantize(None, None, None) == 1
