@@ -15,8 +15,20 @@ namespace {
 constexpr int kThreads = 256;
 
 // eight random bytes, zeros from the n-th on
-__device__ __forceinline__ uint2 load_rand8(const uint8_t* p, int n, bool vec) {
+__device__ __forceinline__ uint2 load_rand8(const uint8_t* p, int n, bool vec, const uint8_t* lo,
+                                            const uint8_t* hi) {
   if (vec && n >= 8) return __ldg(reinterpret_cast<const uint2*>(p));
+  if (n >= 8) {
+    // off 8 bytes: two aligned words, both within [lo, hi), shifted together
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), m = at & 7;
+    const uint2* q = reinterpret_cast<const uint2*>(at - m);
+    if (q >= static_cast<const void*>(lo) && q + 2 <= static_cast<const void*>(hi)) {
+      const uint2 x = __ldg(q), y = __ldg(q + 1);
+      const uint32_t a = m & 4 ? x.y : x.x, b = m & 4 ? y.x : x.y, c = m & 4 ? y.y : y.x;
+      const uint32_t bits = (uint32_t)(m & 3) * 8;
+      return make_uint2(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits));
+    }
+  }
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -36,18 +48,41 @@ struct Rand16 {
   uint2 h[2];
 };
 
+// Elements [0, n) of the 16 at p.  Rows off 16 bytes are read in aligned words where
+// those lie within the matrix, [a.in, its last element].
 template <typename T>
-__device__ __forceinline__ Raw16<T> load16(const T* p, int n, bool vec) {
+__device__ __forceinline__ Raw16<T> load16(const BlockQuantArgs& a, const T* p, int n) {
   Raw16<T> r;
-  r.h[0] = load8(p, n < 8 ? n : 8, vec);
-  r.h[1] = load8(p + 8, n < 8 ? 0 : n - 8, vec);
+  if (!a.in_vec && n == 16) {
+    const T* lo = static_cast<const T*>(a.in);
+    const T* hi = lo + ((a.rows - 1) * a.ld_in + a.cols);
+    uint32_t u[8], v[8];
+    if constexpr (sizeof(T) == 2) {
+      if (load32_any(p, lo, hi, u)) {
+        r.h[0].w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        r.h[1].w[0] = make_uint4(u[4], u[5], u[6], u[7]);
+        return r;
+      }
+    } else {
+      if (load32_any(p, lo, hi, u) && load32_any(p + 8, lo, hi, v)) {
+        r.h[0].w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        r.h[0].w[1] = make_uint4(u[4], u[5], u[6], u[7]);
+        r.h[1].w[0] = make_uint4(v[0], v[1], v[2], v[3]);
+        r.h[1].w[1] = make_uint4(v[4], v[5], v[6], v[7]);
+        return r;
+      }
+    }
+  }
+  r.h[0] = load8(p, n < 8 ? n : 8, a.in_vec);
+  r.h[1] = load8(p + 8, n < 8 ? 0 : n - 8, a.in_vec);
   return r;
 }
 
-__device__ __forceinline__ Rand16 load_rand16(const uint8_t* p, int n, bool vec) {
+__device__ __forceinline__ Rand16 load_rand16(const BlockQuantArgs& a, const uint8_t* p, int n) {
   Rand16 r;
-  r.h[0] = load_rand8(p, n < 8 ? n : 8, vec);
-  r.h[1] = load_rand8(p + 8, n < 8 ? 0 : n - 8, vec);
+  const uint8_t* hi = a.rand + ((a.rows - 1) * a.ld_rand + a.cols);
+  r.h[0] = load_rand8(p, n < 8 ? n : 8, a.rand_vec, a.rand, hi);
+  r.h[1] = load_rand8(p + 8, n < 8 ? 0 : n - 8, a.rand_vec, a.rand, hi);
   return r;
 }
 
@@ -109,13 +144,13 @@ __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const BlockQuantAr
        r += 2 * step) {
     const bool ok0 = in_row && r < a.rows, ok1 = in_row && r + step < a.rows;
     const T* p = static_cast<const T*>(a.in) + r * a.ld_in + c;
-    const Raw16<T> raw0 = load16(p, ok0 ? n : 0, a.in_vec);
-    const Raw16<T> raw1 = load16(p + step * a.ld_in, ok1 ? n : 0, a.in_vec);
+    const Raw16<T> raw0 = load16(a, p, ok0 ? n : 0);
+    const Raw16<T> raw1 = load16(a, p + step * a.ld_in, ok1 ? n : 0);
     Rand16 rnd0, rnd1;
     if constexpr (SR) {
       const uint8_t* q = a.rand + r * a.ld_rand + c;
-      rnd0 = load_rand16(q, ok0 ? n : 0, a.rand_vec);
-      rnd1 = load_rand16(q + step * a.ld_rand, ok1 ? n : 0, a.rand_vec);
+      rnd0 = load_rand16(a, q, ok0 ? n : 0);
+      rnd1 = load_rand16(a, q + step * a.ld_rand, ok1 ? n : 0);
     }
     encode_row16<T, FMT, QM, SR, PRE>(raw0, a.scale, rnd0, a.codes + (r * a.kp + c) * bits / 8,
                                       a.sf + (r * a.kp + c) / blk, ok0);
@@ -155,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantAr
     const int item = i * kThreads + tid;
     const int64_t r = r0 + item / kVec, c = c0 + item % kVec * 16;
     const int n = r >= a.rows || c >= a.cols ? 0 : (int)(a.cols - c < 16 ? a.cols - c : 16);
-    raw[i] = load16(static_cast<const T*>(a.in) + r * a.ld_in + c, n, a.in_vec);
+    raw[i] = load16(a, static_cast<const T*>(a.in) + r * a.ld_in + c, n);
   }
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
@@ -165,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantAr
     Rand16 rnd;
     if constexpr (SR) {
       const int n = r >= a.rows || c >= a.cols ? 0 : (int)(a.cols - c < 16 ? a.cols - c : 16);
-      rnd = load_rand16(a.rand + r * a.ld_rand + c, n, a.rand_vec);
+      rnd = load_rand16(a, a.rand + r * a.ld_rand + c, n);
       // pair p of 32-bit words of a row lies at p ^ g (fp32 tiles: half as many pairs)
       uint2* q = reinterpret_cast<uint2*>(rnd_tile) + lr * (kRandWords / 2);
       q[(2 * v) ^ (g & (kRandWords / 2 - 1))] = rnd.h[0];
@@ -262,53 +297,108 @@ __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantAr
 }
 
 // Read-back: eight codes per thread, of four rows at a time so that their loads are in
-// flight together.
-template <typename T, int FMT>
+// flight together.  SHIFT: rows of `out` off 16 bytes; a thread then takes the eight
+// elements of an aligned place in the row, whose codes are shifted out of two words and
+// which may meet two blocks.
+template <typename T, int FMT, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(const BlockDequantArgs a) {
-  constexpr int bits = bf_bits(FMT), blk = bf_block(FMT), kRows = 4;
-  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
-  if (c >= a.cols) return;
-  const int n = (int)(a.cols - c < 8 ? a.cols - c : 8);
-  const int64_t step = (int64_t)gridDim.y * blockDim.y;
+  constexpr int blk = bf_block(FMT), kRows = 4, kWords = bf_bits(FMT) / 4;  // words of eight codes
+  const int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t step = (int64_t)gridDim.y * blockDim.y, last = a.kp / 8 - 1;
   for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows * step) {
-    uint2 w[kRows];
-    uint32_t sb[kRows];
+    uint32_t w[kRows][SHIFT ? 2 * kWords : kWords];
+    uint32_t sb[kRows][SHIFT ? 2 : 1];
+    int64_t c[kRows];
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int64_t r = r0 + k * step, e = (r < a.rows ? r : r0) * a.kp + c;
-      if constexpr (FMT == BF_MXF8)
-        w[k] = __ldg(reinterpret_cast<const uint2*>(a.codes + e));
-      else
-        w[k].x = __ldg(reinterpret_cast<const uint32_t*>(a.codes + e * bits / 8));
-      sb[k] = __ldg(a.sf + e / blk);
+      const int64_t r = r0 + k * step < a.rows ? r0 + k * step : r0;
+      c[k] = v * 8;
+      if constexpr (SHIFT) {
+        // elements of the row before its first aligned place
+        const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<T*>(a.out) + r * a.ld_out);
+        const int lead = (int)((16 - (at & 15)) & 15) / (int)sizeof(T);
+        c[k] = lead ? v * 8 + lead - 8 : v * 8;
+      }
+      // eights of codes: the one c lies in (or the row's ends where there is none), the next
+      int64_t e = c[k] < 0 ? 0 : c[k] / 8;
+      e = e < last ? e : last;
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.codes) + (r * (a.kp / 8) + e) * kWords;
+      const uint8_t* sf = a.sf + r * (a.kp / blk);
+      const int next = e < last ? 1 : 0;
+      if constexpr (kWords == 2) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+        w[k][0] = x.x;
+        w[k][1] = x.y;
+        if constexpr (SHIFT) {
+          const uint2 y = __ldg(reinterpret_cast<const uint2*>(p) + next);
+          w[k][2] = y.x;
+          w[k][3] = y.y;
+        }
+      } else {
+        w[k][0] = __ldg(p);
+        if constexpr (SHIFT) w[k][1] = __ldg(p + next);
+      }
+      sb[k][0] = __ldg(sf + e * 8 / blk);
+      if constexpr (SHIFT) sb[k][1] = __ldg(sf + (e + next) * 8 / blk);
     }
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
       const int64_t r = r0 + k * step;
-      if (r >= a.rows) break;
-      float s;
-      if constexpr (FMT == BF_NVFP4)
-        s = e4m3_pair(sb[k]).x;
-      else
-        s = e8m0_value(sb[k]);
-      float2 v[4];
+      if (r >= a.rows || c[k] >= a.cols) continue;
+      auto scale_of = [](uint32_t b) { return FMT == BF_NVFP4 ? e4m3_pair(b).x : e8m0_value(b); };
+      const float s0 = scale_of(sb[k][0]);
+      // codes from c[k] on: c[k] < 0 starts before the row, with places that are not stored
+      int part = 0;  // elements of the first eight that come before
+      uint32_t u[kWords];
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) u[i] = w[k][i];
+      float s1 = s0;
+      if constexpr (SHIFT) {
+        part = (int)(c[k] & 7);
+        s1 = scale_of(sb[k][1]);
+        if (c[k] < 0) {  // the first eight stand where the second would
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            w[k][i + kWords] = w[k][i];
+            w[k][i] = 0u;
+          }
+          s1 = s0;
+        }
+        if constexpr (kWords == 1) {
+          u[0] = __funnelshift_r(w[k][0], w[k][1], 4 * part);
+        } else {
+          const uint32_t x = part & 4 ? w[k][1] : w[k][0], y = part & 4 ? w[k][2] : w[k][1],
+                         z = part & 4 ? w[k][3] : w[k][2];
+          u[0] = __funnelshift_r(x, y, 8 * (part & 3));
+          u[1] = __funnelshift_r(y, z, 8 * (part & 3));
+        }
+      }
+      float2 f[4];
       if constexpr (FMT == BF_MXF8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = e4m3_pair((i < 2 ? w[k].x : w[k].y) >> (16 * (i & 1)));
+        for (int i = 0; i < 4; ++i) f[i] = e4m3_pair(u[i >> 1] >> (16 * (i & 1)));
       } else {
         uint32_t h[4];
-        e2m1x8_pairs(w[k].x, h);
+        e2m1x8_pairs(u[0], h);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
       }
       // code * s is exact
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], both(s));
-      if (a.scale != 1.0f)
+      for (int i = 0; i < 4; ++i) {
+        f[i] = mul2(f[i], make_float2(2 * i + part < 8 ? s0 : s1, 2 * i + 1 + part < 8 ? s0 : s1));
+        if (a.scale != 1.0f) f[i] = mul2(f[i], both(a.scale));
+      }
+      const float o[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
+      T* dst = static_cast<T*>(a.out) + r * a.ld_out + c[k];
+      const int64_t left = a.cols - c[k];
+      if (SHIFT && c[k] < 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], both(a.scale));
-      const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-      store8(static_cast<T*>(a.out) + r * a.ld_out + c, f, n, a.out_vec);
+        for (int i = 0; i < 8; ++i)
+          if (c[k] + i >= 0 && i < left) dst[i] = from_f32<T>(o[i]);
+      } else {
+        store8(dst, o, left < 8 ? (int)left : 8, true);
+      }
     }
   }
 }
@@ -367,17 +457,23 @@ cudaError_t quant_fmt(int fmt, bool pow2, const BlockQuantArgs& a, cudaStream_t 
   return quant_sr<T, BF_NVFP4, Q_DIVIDE, true>(a, s);
 }
 
-template <typename T>
+template <typename T, bool SHIFT>
 cudaError_t dequant_fmt(int fmt, const BlockDequantArgs& a, cudaStream_t s) {
   dim3 grid, block;
-  row_shape((a.rows + 3) / 4, a.cols, 8, &grid, &block);
+  // SHIFT: a row may begin before an aligned place
+  row_shape((a.rows + 3) / 4, a.cols + (SHIFT ? 7 : 0), 8, &grid, &block);
   if (fmt == BF_MXF8)
-    dequant_kernel<T, BF_MXF8><<<grid, block, 0, s>>>(a);
+    dequant_kernel<T, BF_MXF8, SHIFT><<<grid, block, 0, s>>>(a);
   else if (fmt == BF_MXF4)
-    dequant_kernel<T, BF_MXF4><<<grid, block, 0, s>>>(a);
+    dequant_kernel<T, BF_MXF4, SHIFT><<<grid, block, 0, s>>>(a);
   else
-    dequant_kernel<T, BF_NVFP4><<<grid, block, 0, s>>>(a);
+    dequant_kernel<T, BF_NVFP4, SHIFT><<<grid, block, 0, s>>>(a);
   return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dequant_rows(int fmt, const BlockDequantArgs& a, cudaStream_t s) {
+  return a.out_vec ? dequant_fmt<T, false>(fmt, a, s) : dequant_fmt<T, true>(fmt, a, s);
 }
 
 }  // namespace
@@ -390,9 +486,9 @@ cudaError_t launch_block_quant(int fmt, int type, bool pow2, const BlockQuantArg
 }
 
 cudaError_t launch_block_dequant(int fmt, int type, const BlockDequantArgs& a, cudaStream_t s) {
-  if (type == B2G_F32) return dequant_fmt<float>(fmt, a, s);
-  if (type == B2G_BF16) return dequant_fmt<__nv_bfloat16>(fmt, a, s);
-  return dequant_fmt<__half>(fmt, a, s);
+  if (type == B2G_F32) return dequant_rows<float>(fmt, a, s);
+  if (type == B2G_BF16) return dequant_rows<__nv_bfloat16>(fmt, a, s);
+  return dequant_rows<__half>(fmt, a, s);
 }
 
 }  // namespace b2g

@@ -83,6 +83,27 @@ __device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec) {
   return r;
 }
 
+// The 32 bytes at p, which has the alignment of its elements only: three aligned 16-byte
+// words, all within [lo, hi), shifted together.  False where they are not within.
+__device__ __forceinline__ bool load32_any(const void* p, const void* lo, const void* hi,
+                                           uint32_t (&u)[8]) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), m = at & 15;
+  const uint4* a = reinterpret_cast<const uint4*>(at - m);
+  if (a < lo || a + 3 > hi) return false;
+  const uint4 x = __ldg(a), y = __ldg(a + 1), z = __ldg(a + 2);
+  uint32_t w[12] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+  if (m & 8)
+#pragma unroll
+    for (int i = 0; i < 10; ++i) w[i] = w[i + 2];
+  if (m & 4)
+#pragma unroll
+    for (int i = 0; i < 9; ++i) w[i] = w[i + 1];
+  const uint32_t bits = (uint32_t)(m & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  return true;
+}
+
 template <typename T>
 __device__ __forceinline__ float2 pair_f32(uint32_t w);
 template <>
