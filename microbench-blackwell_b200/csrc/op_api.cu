@@ -209,11 +209,12 @@ b2g_status b2g_residual_norm(b2g_handle* h, const b2g_residual_norm_desc* d, voi
   a.eps = d->eps;
   a.alpha = d->alpha;
   a.beta = d->beta;
-  a.vec = rows_aligned(d->x, d->ld_x, es, 16) && (!d->y || rows_aligned(d->y, d->ld_y, es, 16)) &&
-          (!d->x_out || rows_aligned(d->x_out, d->ld_x_out, es, 16)) &&
-          (!d->h || rows_aligned(d->h, d->ld_h, es, 16)) &&
-          (!d->gate || rows_aligned(d->gate, d->cols, es, 16)) && aligned(d->w_post, 16) &&
-          aligned(d->w_pre, 16);
+  auto fits = [&](size_t bytes) {
+    auto ok = [&](const void* p, int64_t ld) { return !p || rows_aligned(p, ld, es, bytes); };
+    return ok(d->x, d->ld_x) && ok(d->y, d->ld_y) && ok(d->x_out, d->ld_x_out) && ok(d->h, d->ld_h) &&
+           ok(d->gate, d->cols) && aligned(d->w_post, bytes) && aligned(d->w_pre, bytes);
+  };
+  a.vec = fits(16);
   DeviceGuard g(h->device);
   B2G_CUDA(h, launch_residual_norm(type, h_fmt, a, h->sm_count,
                                    reinterpret_cast<cudaStream_t>(stream)));
@@ -296,11 +297,13 @@ b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_norm_gra
   a.dw_pre = d->dw_pre;
   a.alpha = d->alpha;
   a.beta = d->beta;
-  auto vec = [&](const void* p, int64_t ld) { return !p || rows_aligned(p, ld, es, 16); };
-  a.vec = vec(d->dh, d->ld_dh) && vec(d->dx_out, d->ld_dx_out) &&
-          (!d->dh || vec(d->x_out, d->ld_x_out)) && vec(d->y, d->ld_y) && vec(d->dx, d->ld_dx) &&
-          vec(d->dy, d->ld_dy) && vec(d->gate, d->cols) && aligned(d->w_post, 16) &&
-          aligned(d->w_pre, 16);
+  auto fits = [&](size_t bytes) {
+    auto ok = [&](const void* p, int64_t ld) { return !p || rows_aligned(p, ld, es, bytes); };
+    return ok(d->dh, d->ld_dh) && ok(d->dx_out, d->ld_dx_out) && (!d->dh || ok(d->x_out, d->ld_x_out)) &&
+           ok(d->y, d->ld_y) && ok(d->dx, d->ld_dx) && ok(d->dy, d->ld_dy) && ok(d->gate, d->cols) &&
+           aligned(d->w_post, bytes) && aligned(d->w_pre, bytes);
+  };
+  a.vec = fits(16);
   a.dgate_vec = aligned(d->dgate, 16);
   a.err = h->d_err;
   const b2g_status st = grow(h, norm_grad_ws_bytes(type, a, h->sm_count), 0, s);

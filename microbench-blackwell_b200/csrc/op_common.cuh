@@ -210,6 +210,99 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n, bool ve
     if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
+// Bytes m .. m + 15 of two 16-byte words, m even and below 16.
+__device__ __forceinline__ uint4 shift16(const uint4& x, const uint4& y, uint32_t m) {
+  uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  if (m & 8)
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (m & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const uint32_t bits = (m & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// load8 for rows of any alignment (ANY; else every p is 16-byte aligned): aligned words
+// shifted together where they lie within the operand [lo, hi), else element by element.
+template <typename T, bool ANY>
+__device__ __forceinline__ Raw8<T> load8_any(const T* p, int n, const T* lo, const T* hi) {
+  if constexpr (ANY) {
+    const uint32_t m = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+    if (m && n >= 8) {
+      Raw8<T> r;
+      if constexpr (sizeof(T) == 4) {
+        uint32_t u[8];
+        if (load32_any(p, lo, hi, u)) {
+          r.w[0] = make_uint4(u[0], u[1], u[2], u[3]);
+          r.w[1] = make_uint4(u[4], u[5], u[6], u[7]);
+          return r;
+        }
+      } else {
+        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - m);
+        if (q >= static_cast<const void*>(lo) && q + 2 <= static_cast<const void*>(hi)) {
+          r.w[0] = shift16(__ldg(q), __ldg(q + 1), m);
+          return r;
+        }
+      }
+      return load8(p, n, false);
+    }
+    return load8(p, n, m == 0);
+  } else {
+    return load8(p, n, true);
+  }
+}
+
+// store8 of a whole warp for rows of any alignment (ANY): p is lane 0's place plus eight
+// elements a lane, `count` the warp's elements in the row.  The values go through `buf`
+// (the warp's own, (8 * sizeof(T)) * 32 + 16 bytes) and out as aligned 16-byte words, with
+// single elements at the ends.
+template <typename T, bool ANY>
+__device__ __forceinline__ void store8_any(T* p, const float (&v)[8], int n, int count, uint4* buf) {
+  if constexpr (!ANY) {
+    store8(p, v, n, true);
+  } else {
+    constexpr int W = (int)sizeof(T) / 2;  // 16-byte words of eight elements
+    const int lane = threadIdx.x & 31;
+    T* first = p - lane * 8;
+    const uint32_t m = (uint32_t)reinterpret_cast<uintptr_t>(first) & 15u;
+    if (m == 0) {
+      store8(p, v, n, true);
+      return;
+    }
+    if constexpr (sizeof(T) == 4) {
+      buf[lane * 2] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                 __float_as_uint(v[3]));
+      buf[lane * 2 + 1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]),
+                                     __float_as_uint(v[6]), __float_as_uint(v[7]));
+    } else {
+      buf[lane] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                             pack2<T>(v[6], v[7]));
+    }
+    __syncwarp();
+    const int bytes = count * (int)sizeof(T);
+    int head = 16 - (int)m;
+    head = head < bytes ? head : bytes;
+    const int full = (bytes - head) / 16;
+    char* dst = reinterpret_cast<char*>(first);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const int i = k * 32 + lane;
+      if (i < full)
+        *reinterpret_cast<uint4*>(dst + head + 16 * i) = shift16(buf[i], buf[i + 1], 16 - m);
+    }
+    // elements before the first word and after the last
+    const int tail = head + 16 * full, heads = head / (int)sizeof(T);
+    const int rest = (bytes - tail) / (int)sizeof(T);
+    const T* e = reinterpret_cast<const T*>(buf);
+    if (lane < heads) first[lane] = e[lane];
+    if (lane >= 16 && lane - 16 < rest)
+      first[tail / (int)sizeof(T) + lane - 16] = e[tail / (int)sizeof(T) + lane - 16];
+    __syncwarp();
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void store4x2(T* p, const float2 (&v)[4], bool vec) {
   const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};

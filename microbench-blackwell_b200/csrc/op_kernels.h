@@ -63,7 +63,7 @@ struct ResidualNormGradArgs {
   void *dx, *dy;
   float *dgate, *dw_post, *dw_pre;
   float alpha, beta;
-  int vec;
+  int vec;        // as above
   int dgate_vec;  // dgate starts on 16 bytes
   uint32_t* err;  // the handle's error word
   void* ws;  // norm_grad_ws_bytes() bytes

@@ -39,25 +39,39 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* red) {
 }
 
 // One row per blockDim.x threads, held in registers: NV times eight elements a thread.
-template <typename T, int NV, int HF>
+// ANY: operands of any alignment.
+template <typename T, int NV, int HF, bool ANY>
 __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormArgs a) {
   __shared__ float red[2][32];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= a.rows) return;  // whole warps: blockDim.y > 1 only with one warp per row
-  const bool vec = a.vec;
-  const int64_t width = HF < 0 ? a.cols : a.kp;
+  extern __shared__ __align__(16) uint4 stores[];  // ANY: one buffer a warp
+  uint4* buf = stores + (threadIdx.y * blockDim.x + threadIdx.x) / 32 * (2 * sizeof(T) * 8 + 1);
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const T* y = static_cast<const T*>(a.y) + row * a.ld_y;
   Raw8<T> rx[NV], ry[NV];
-  int n[NV];
-  int64_t col[NV];
+  const int cols = (int)a.cols;
+  int col[NV], n[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    col[j] = ((int64_t)j * blockDim.x + threadIdx.x) * 8;
-    const int64_t left = a.cols - col[j];
-    n[j] = left < 0 ? 0 : left < 8 ? (int)left : 8;
-    rx[j] = load8(x + col[j], n[j], vec);
-    if (a.y) ry[j] = load8(y + col[j], n[j], vec);
+    col[j] = (j * (int)blockDim.x + (int)threadIdx.x) * 8;
+    const int left = cols - col[j];
+    n[j] = left < 0 ? 0 : left < 8 ? left : 8;
+  }
+  // eight elements of a row of an operand that has `rows` rows, ld apart
+  auto get = [&](const void* p, const T* row, int64_t rows, int64_t ld, int j) {
+    const T* lo = static_cast<const T*>(p);
+    return load8_any<T, ANY>(row + col[j], n[j], lo, lo + ((rows - 1) * ld + cols));
+  };
+  auto put = [&](void* p, int64_t ld, int j, const float(&f)[8]) {
+    const int left = cols - (col[j] - (int)(threadIdx.x & 31) * 8);
+    store8_any<T, ANY>(static_cast<T*>(p) + row * ld + col[j], f, n[j],
+                       left < 0 ? 0 : left < 256 ? left : 256, buf);
+  };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    rx[j] = get(a.x, x, a.rows, a.ld_x, j);
+    if (a.y) ry[j] = get(a.y, y, a.rows, a.ld_y, j);
   }
   float v[NV][8];
   if (a.y) {
@@ -83,13 +97,13 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
       unpack8(ry[j], fy);
       if (a.w_post) {
         float w[8];
-        unpack8(load8(static_cast<const T*>(a.w_post) + col[j], n[j], vec), w);
+        unpack8(get(a.w_post, static_cast<const T*>(a.w_post), 1, 0, j), w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) fy[i] = fy[i] * r1 * w[i];
       }
       if (gate) {
         float g[8];
-        unpack8(load8(gate + col[j], n[j], vec), g);
+        unpack8(get(a.gate, gate, (a.rows - 1) / a.rows_per_gate + 1, a.cols, j), g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) fy[i] *= g[i];
       }
@@ -107,7 +121,7 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
   if (a.x_out) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      store8(static_cast<T*>(a.x_out) + row * a.ld_x_out + col[j], v[j], n[j], vec);
+      put(a.x_out, a.ld_x_out, j, v[j]);
   }
   if (!a.w_pre) return;
   float ss[1] = {0.0f};
@@ -121,10 +135,10 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     float w[8];
-    unpack8(load8(static_cast<const T*>(a.w_pre) + col[j], n[j], vec), w);
+    unpack8(get(a.w_pre, static_cast<const T*>(a.w_pre), 1, 0, j), w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * r2 * w[i];
-    if (a.h) store8(static_cast<T*>(a.h) + row * a.ld_h + col[j], v[j], n[j], vec);
+    if (a.h) put(a.h, a.ld_h, j, v[j]);
     if constexpr (HF >= 0) {
       constexpr int blk = bf_block(HF), bits = bf_bits(HF);
       constexpr int mode = HF == BF_NVFP4 ? Q_DIVIDE : Q_EXACT;
@@ -138,7 +152,7 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
                             make_float2(v[j][4], v[j][5]), make_float2(v[j][6], v[j][7])};
       uint32_t q[2];
       encode8<HF, mode, false>(x2, s, 1.0f, make_uint2(0, 0), q);
-      if (col[j] < width) {
+      if (col[j] < a.kp) {
         const int64_t e = row * a.kp + col[j];
         if constexpr (HF == BF_MXF8)
           *reinterpret_cast<uint2*>(a.codes + e) = make_uint2(q[0], q[1]);
@@ -150,35 +164,31 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
   }
 }
 
-template <typename T, int HF>
+template <typename T, int HF, bool ANY>
 cudaError_t norm_launch(const ResidualNormArgs& a, int sm_count, cudaStream_t s) {
   const int64_t v = ((HF < 0 ? a.cols : a.kp) + 7) / 8;
   // few rows: as many threads to a row as it has eights, for latency; many: four eights
   // a thread, which keeps eight 16-byte loads in flight in each
-  const int want = a.rows < 2 * sm_count ? 1 : 4;
-  int nv = 1;
-  while (nv < 4 && (nv < want || (v + nv - 1) / nv > 1024)) nv *= 2;
+  const int nv = a.rows < 2 * sm_count && v <= 1024 ? 1 : 4;
   int64_t tpr = ((v + nv - 1) / nv + 31) / 32 * 32;
-  if (tpr < 32) tpr = 32;
   const int rpc = tpr == 32 ? 4 : 1;
   const dim3 block((unsigned)tpr, rpc);
   const unsigned grid = (unsigned)((a.rows + rpc - 1) / rpc);
+  const size_t smem = ANY ? tpr * rpc / 32 * (2 * sizeof(T) * 8 + 1) * sizeof(uint4) : 0;
   if (nv == 1)
-    residual_norm_kernel<T, 1, HF><<<grid, block, 0, s>>>(a);
-  else if (nv == 2)
-    residual_norm_kernel<T, 2, HF><<<grid, block, 0, s>>>(a);
+    residual_norm_kernel<T, 1, HF, ANY><<<grid, block, smem, s>>>(a);
   else
-    residual_norm_kernel<T, 4, HF><<<grid, block, 0, s>>>(a);
+    residual_norm_kernel<T, 4, HF, ANY><<<grid, block, smem, s>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t norm_fmt(int h_fmt, const ResidualNormArgs& a, int sm_count, cudaStream_t s) {
   switch (h_fmt) {
-    case BF_NVFP4: return norm_launch<T, BF_NVFP4>(a, sm_count, s);
-    case BF_MXF4: return norm_launch<T, BF_MXF4>(a, sm_count, s);
-    case BF_MXF8: return norm_launch<T, BF_MXF8>(a, sm_count, s);
-    default: return norm_launch<T, -1>(a, sm_count, s);
+    case BF_NVFP4: return a.vec ? norm_launch<T, BF_NVFP4, false>(a, sm_count, s) : norm_launch<T, BF_NVFP4, true>(a, sm_count, s);
+    case BF_MXF4: return a.vec ? norm_launch<T, BF_MXF4, false>(a, sm_count, s) : norm_launch<T, BF_MXF4, true>(a, sm_count, s);
+    case BF_MXF8: return a.vec ? norm_launch<T, BF_MXF8, false>(a, sm_count, s) : norm_launch<T, BF_MXF8, true>(a, sm_count, s);
+    default: return a.vec ? norm_launch<T, -1, false>(a, sm_count, s) : norm_launch<T, -1, true>(a, sm_count, s);
   }
 }
 
@@ -577,24 +587,29 @@ cudaError_t grad_rows_launch(const ResidualNormGradArgs& a, const GradRows& p, c
 
 // Row means: stat[row] = {r2^3 A / D, r1^3 (B - r2^3 (A / D) C) / D} (the second r1-free
 // without w_post: 0).
-template <typename T>
+template <typename T, bool ANY>
 __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradArgs a, float2* stat) {
   __shared__ float red[3 * 32];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= a.rows) return;
-  const bool vec = a.vec;
+  const int span = blockDim.x;
   const float r2 = a.dh ? a.rstd_pre[row] : 0.0f;
   const float r1 = a.w_post ? a.rstd_post[row] : 0.0f;
-  const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
   float s[3] = {0.0f, 0.0f, 0.0f};
-  for (int64_t c = threadIdx.x * 8; c < a.cols; c += blockDim.x * 8) {
-    const int n = a.cols - c < 8 ? (int)(a.cols - c) : 8;
+  const int cols = (int)a.cols;
+  for (int c = threadIdx.x * 8; c < cols; c += span * 8) {
+    const int n = cols - c < 8 ? cols - c : 8;
+    // columns c .. of row r of an operand with `rows` rows, ld apart
+    auto get = [&](const void* p, int64_t r, int64_t ld, int64_t rows, float (&f)[8]) {
+      const T* lo = static_cast<const T*>(p);
+      unpack8(load8_any<T, ANY>(lo + r * ld + c, n, lo, lo + ((rows - 1) * ld + cols)), f);
+    };
     float p[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (a.dh) {
       float w[8];
-      unpack8(load8(static_cast<const T*>(a.dh) + row * a.ld_dh + c, n, vec), p);
-      unpack8(load8(static_cast<const T*>(a.v) + row * a.ld_v + c, n, vec), v);
-      unpack8(load8(static_cast<const T*>(a.w_pre) + c, n, vec), w);
+      get(a.dh, row, a.ld_dh, a.rows, p);
+      get(a.v, row, a.ld_v, a.rows, v);
+      get(a.w_pre, 0, 0, 1, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] *= w[i];
@@ -603,12 +618,12 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradAr
     }
     if (a.w_post) {
       float y[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      unpack8(load8(static_cast<const T*>(a.y) + row * a.ld_y + c, n, vec), y);
-      unpack8(load8(static_cast<const T*>(a.w_post) + c, n, vec), w);
-      if (a.dx_out) unpack8(load8(static_cast<const T*>(a.dx_out) + row * a.ld_dx_out + c, n, vec), d);
-      if (gate) {
+      get(a.y, row, a.ld_y, a.rows, y);
+      get(a.w_post, 0, 0, 1, w);
+      if (a.dx_out) get(a.dx_out, row, a.ld_dx_out, a.rows, d);
+      if (a.gate) {
         float g[8];
-        unpack8(load8(gate + c, n, vec), g);
+        get(a.gate, row / a.rows_per_gate, a.cols, (a.rows - 1) / a.rows_per_gate + 1, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] *= g[i];
       }
@@ -664,15 +679,25 @@ GradChunks grad_chunks(const ResidualNormGradArgs& a, int sm_count) {
 
 // Column pass: 256 columns (eight a thread) of one chunk of rows, a row per warp.  Sums
 // over the chunk go to part[chunk][3][cols] (dw_pre, dw_post, dgate).
-template <typename T>
+template <typename T, bool ANY>
 __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradArgs a, GradChunks ck,
                                                         const float2* stat, float* part) {
   __shared__ float red[kLanes][kGradCols];
   const int lane = threadIdx.x, ry = threadIdx.y;
   const int64_t chunk = blockIdx.x;
-  const int64_t c = (int64_t)blockIdx.y * kGradCols + lane * 8;
-  const int n = c >= a.cols ? 0 : a.cols - c < 8 ? (int)(a.cols - c) : 8;
-  const bool vec = a.vec;
+  __shared__ uint4 gate_stores[kLanes][65];
+  __shared__ uint4 stores[ANY ? kLanes : 1][2 * sizeof(T) * 8 + 1];
+  const int cols = (int)a.cols, c0 = (int)blockIdx.y * kGradCols, c = c0 + lane * 8;
+  const int n = c >= cols ? 0 : cols - c < 8 ? cols - c : 8;
+  const int count = cols - c0 < 256 ? cols - c0 : 256;
+  // columns c .. of row r of an operand with `rows` rows, ld apart
+  auto get = [&](const void* p, int64_t r, int64_t ld, int64_t rows, float (&f)[8]) {
+    const T* lo = static_cast<const T*>(p);
+    unpack8(load8_any<T, ANY>(lo + r * ld + c, n, lo, lo + ((rows - 1) * ld + cols)), f);
+  };
+  auto put = [&](void* p, int64_t r, int64_t ld, const float(&f)[8]) {
+    store8_any<T, ANY>(static_cast<T*>(p) + r * ld + c, f, n, count, stores[ANY ? ry : 0]);
+  };
   int64_t r0, r1;
   if (ck.whole) {
     r0 = chunk * ck.rows;
@@ -684,8 +709,8 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
   }
   if (r1 > a.rows) r1 = a.rows;
   float wq[8], wp[8], g[8];
-  if (a.w_post) unpack8(load8(static_cast<const T*>(a.w_post) + c, n, vec), wp);
-  if (a.dh) unpack8(load8(static_cast<const T*>(a.w_pre) + c, n, vec), wq);
+  if (a.w_post) get(a.w_post, 0, 0, 1, wp);
+  if (a.dh) get(a.w_pre, 0, 0, 1, wq);
   float dwq[8], dwp[8], dg[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -699,16 +724,16 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
   for (int64_t rb = r0 + ry * run; rb < r1; rb += kLanes * run) {
     const int64_t re = rb + run < r1 ? rb + run : r1;
     if (a.gate && (ck.whole || rb == r0 + ry * run))
-      unpack8(load8(static_cast<const T*>(a.gate) + rb / ck.per * a.cols + c, n, vec), g);
+      get(a.gate, rb / ck.per, a.cols, ck.gates, g);
     for (int64_t r = rb; r < re; ++r) {
       const float2 st = stat[r];
       float dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (a.dx_out) unpack8(load8(static_cast<const T*>(a.dx_out) + r * a.ld_dx_out + c, n, vec), dv);
+      if (a.dx_out) get(a.dx_out, r, a.ld_dx_out, a.rows, dv);
       if (a.dh) {
         const float r2 = a.rstd_pre[r];
         float dh[8], v[8];
-        unpack8(load8(static_cast<const T*>(a.dh) + r * a.ld_dh + c, n, vec), dh);
-        unpack8(load8(static_cast<const T*>(a.v) + r * a.ld_v + c, n, vec), v);
+        get(a.dh, r, a.ld_dh, a.rows, dh);
+        get(a.v, r, a.ld_v, a.rows, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           dv[i] += r2 * wq[i] * dh[i] - v[i] * st.x;
@@ -719,12 +744,12 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
       if (a.dx) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = a.alpha * dv[i];
-        store8(static_cast<T*>(a.dx) + r * a.ld_dx + c, o, n, vec);
+        put(a.dx, r, a.ld_dx, o);
       }
       if (a.y) {
         const float r1s = a.w_post ? a.rstd_post[r] : 1.0f;
         float y[8];
-        unpack8(load8(static_cast<const T*>(a.y) + r * a.ld_y + c, n, vec), y);
+        get(a.y, r, a.ld_y, a.rows, y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float bd = a.beta * dv[i], yh = y[i] * r1s, dz = bd * g[i];
@@ -732,11 +757,11 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
           dwp[i] = fmaf(dz, yh, dwp[i]);
           o[i] = r1s * wp[i] * dz - y[i] * st.y;
         }
-        if (a.dy) store8(static_cast<T*>(a.dy) + r * a.ld_dy + c, o, n, vec);
+        if (a.dy) put(a.dy, r, a.ld_dy, o);
       }
     }
     if (ck.whole && a.dgate) {
-      store8(a.dgate + rb / ck.per * a.cols + c, dg, n, false);
+      store8_any<float, true>(a.dgate + rb / ck.per * a.cols + c, dg, n, count, gate_stores[ry]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) dg[i] = 0.0f;
     }
@@ -788,10 +813,16 @@ cudaError_t grad_launch(int type, const ResidualNormGradArgs& a, int sm_count, c
   const int64_t v = (a.cols + 7) / 8;
   const int tpr = v <= 32 ? 32 : v <= 64 ? 64 : v <= 128 ? 128 : 256;
   const int rpc = tpr == 32 ? 4 : 1;
-  grad_stat_kernel<T><<<(unsigned)((a.rows + rpc - 1) / rpc), dim3(tpr, rpc), 0, s>>>(a, stat);
+  const unsigned stat_grid = (unsigned)((a.rows + rpc - 1) / rpc);
   const unsigned col_tiles = (unsigned)((a.cols + kGradCols - 1) / kGradCols);
-  grad_cols_kernel<T><<<dim3((unsigned)ck.chunks, col_tiles), dim3(32, kLanes), 0, s>>>(a, ck, stat,
-                                                                                        part);
+  const dim3 cols_grid((unsigned)ck.chunks, col_tiles), cols_block(32, kLanes);
+  if (a.vec) {
+    grad_stat_kernel<T, false><<<stat_grid, dim3(tpr, rpc), 0, s>>>(a, stat);
+    grad_cols_kernel<T, false><<<cols_grid, cols_block, 0, s>>>(a, ck, stat, part);
+  } else {
+    grad_stat_kernel<T, true><<<stat_grid, dim3(tpr, rpc), 0, s>>>(a, stat);
+    grad_cols_kernel<T, true><<<cols_grid, cols_block, 0, s>>>(a, ck, stat, part);
+  }
   const unsigned sums = (unsigned)((a.cols + 31) / 32);
   if (a.dw_pre)
     grad_sum_kernel<<<dim3(1, sums), dim3(32, 8), 0, s>>>(part, 3 * a.cols, ck.chunks, a.cols, a.dw_pre);
