@@ -492,4 +492,41 @@ __device__ __forceinline__ void encode8(const float2 (&x)[4], const BlockScale& 
   }
 }
 
+// ---------------------------------------------------------------- sums
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+// Sums of K values over the CTA's row of threads (blockDim.x of them; one warp per row
+// where blockDim.x is 32).  `red`: K * 32 floats, not in use by an earlier call.
+template <int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if (blockDim.x == 32) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[k * 32 + warp] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? red[k * 32 + lane] : 0.0f);
+}
+
+// The same over a CTA of any number of warps, always with its barrier.
+template <int K>
+__device__ __forceinline__ void row_sum_cta(float (&v)[K], float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[k * 32 + warp] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(lane < warps ? red[k * 32 + lane] : 0.0f);
+}
+
 }  // namespace b2g
