@@ -1,0 +1,562 @@
+// few_tiles.cu -- y = alpha * x . W^T of some tens of tokens with microscaled weights: the
+// tensor-core form of b2g_linear (few_linear.cu has the form for a handful).
+//
+// The weights are the 128-row operand A of tcgen05.mma kind::f16, taken from tensor memory:
+// eight warps decode codes to fp16 (exact, as in few_linear.cu) and write them there, a row
+// a thread, so that decoded weights never pass through shared memory.  x, laid out as fp16
+// by a first kernel, is operand B, up to 128 tokens of it; sums stay in tensor memory until
+// the end.  A decoded weight then serves all tokens for one instruction's issue, and what
+// bounds the kernel is the weights' bytes and their decoding, not the products.
+#include <cuda.h>
+
+#include "b2g.h"
+#include "b2g_desc.h"
+#include "b2g_gemm.h"
+#include "b2g_ptx.cuh"
+#include "op_common.cuh"
+#include "op_kernels.h"
+
+namespace b2g {
+namespace {
+
+constexpr int kRows = 128;            // weight rows of a CTA
+constexpr int kDecodeWarps = 8;       // four for each half of a step
+constexpr int kThreads = (kDecodeWarps + 2) * 32;
+constexpr int kCodeBytes = 128;       // of a row in a step
+constexpr int kMaxStages = 4;
+
+__host__ __device__ constexpr int step_k(int fmt) { return kCodeBytes * 8 / bf_bits(fmt); }
+
+struct TileShape {
+  int tokens;    // of a CTA, a multiple of 16 up to 128
+  int steps;     // of K in all
+  int slices;    // of K, one a CTA
+  int row_tiles, z;
+  int stages;
+  int words;     // a thread's scales of a half step are one aligned word
+  int smem;
+};
+
+// x as fp16 [T][steps * step_k], zero past K, times a power of two for each token (bf16)
+// that brings its largest value to 2^14 .. 2^15; xs[token] undoes it.
+template <typename T>
+__global__ void __launch_bounds__(512) tiles_prepare_kernel(const FewLinearArgs a, int64_t kq,
+                                                            __half* x16, float* xs) {
+  __shared__ float red[16];
+  const int64_t token = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + token * a.ld_x;
+  // the product kernel may start; it waits for this one to end before it reads x
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  float scale = 1.0f;
+  auto eight = [&](int64_t v) {
+    const int64_t left = a.K - v * 8;
+    return load8(x + v * 8, left < 0 ? 0 : left < 8 ? (int)left : 8, a.x_vec);
+  };
+  if constexpr (__is_same(T, __nv_bfloat16)) {
+    float amax = 0.0f;
+    for (int64_t v = threadIdx.x; v * 8 < a.K; v += 512) {
+      float f[8];
+      unpack8(eight(v), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float m = fabsf(f[i]);
+        amax = fmaxf(amax, m < __uint_as_float(0x7F800000u) ? m : 0.0f);  // of the finite ones
+      }
+    }
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(top);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, red[i]);
+    int e = 127 + 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
+    e = e > 253 ? 253 : e;
+    scale = amax > 0.0f ? __uint_as_float((uint32_t)e << 23) : 1.0f;
+  }
+  if (threadIdx.x == 0) xs[token] = 1.0f / scale;
+  for (int64_t v = threadIdx.x; v * 8 < kq; v += 512) {
+    const Raw8<T> r = eight(v);
+    uint4 w = r.w[0];
+    if constexpr (__is_same(T, __nv_bfloat16)) {
+      float f[8];
+      unpack8(r, f);
+      w = make_uint4(pack2<__half>(f[0] * scale, f[1] * scale), pack2<__half>(f[2] * scale, f[3] * scale),
+                     pack2<__half>(f[4] * scale, f[5] * scale), pack2<__half>(f[6] * scale, f[7] * scale));
+    }
+    *reinterpret_cast<uint4*>(x16 + token * kq + v * 8) = w;
+  }
+}
+
+// 32 lanes x 16 columns of 32 bits: lane i of the warp writes TMEM lane (its quarter * 32 + i)
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// A thread's scale bytes of half a step: NVFP4 8, MXFP4 4, MXFP8 2, in the low bytes.
+template <int FMT>
+__device__ __forceinline__ uint2 load_scales(const uint8_t* row, int first, int count, bool words) {
+  constexpr int n = step_k(FMT) / 2 / bf_block(FMT);
+  uint2 s = make_uint2(0u, 0u);
+  if (words) {  // whole and aligned, or past the row's end
+    if (first < count) {
+      if constexpr (n == 8)
+        s = __ldg(reinterpret_cast<const uint2*>(row + first));
+      else if constexpr (n == 4)
+        s.x = __ldg(reinterpret_cast<const uint32_t*>(row + first));
+      else
+        s.x = __ldg(reinterpret_cast<const uint16_t*>(row + first));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t b = first + i < count ? __ldg(row + first + i) : 0u;
+      if (i < 4)
+        s.x |= b << (8 * i);
+      else
+        s.y |= b << (8 * (i - 4));
+    }
+  }
+  return s;
+}
+
+// Rows of the weights' scales within a CTA's K slice share one power of two (MX), the
+// largest scale of the row there: 2^(s - ref) times an element is exact in fp16 down to
+// 2^-14.  A block below that (and not all zeros) is left out of the tensor product and
+// multiplied in fp32 by its own thread, into far[token] of the row.
+template <int FMT>
+__device__ __noinline__ void far_block(const uint32_t (&codes)[4], uint32_t scale, uint32_t x_stage,
+                                       int tokens, int k, float* far) {
+  constexpr int elems = 128 / bf_bits(FMT);
+  const float s = e8m0_value(scale);
+  for (int t = 0; t < tokens; ++t) {
+    float dot = 0.0f;
+    for (int i = 0; i < elems; ++i) {
+      const int kk = k + i, byte = kk % 64 * 2;
+      const uint32_t at = x_stage + (kk / 64 * tokens + t) * 128 + (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15);
+      uint16_t h;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
+      const uint32_t word = codes[i * bf_bits(FMT) / 32] >> (i * bf_bits(FMT) % 32);
+      float c;
+      if constexpr (FMT == BF_MXF8) {
+        c = e4m3_pair(word & 0xFFu).x;
+      } else {
+        uint32_t p[4];
+        e2m1x8_pairs(word & 15u, p);
+        c = __half2float(__ushort_as_half((unsigned short)(p[0] & 0xFFFFu)));
+      }
+      dot = fmaf(c, __half2float(__ushort_as_half(h)), dot);
+    }
+    far[t] = fmaf(s, dot, far[t]);
+  }
+}
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads, 1)
+few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                 const FewLinearArgs a, const TileShape sh, const float* xs, float* part, float* far_ws) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  // ring slots (codes, then x) start on 1024 bytes
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4 + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int aborted;
+  __shared__ bool last;
+  __shared__ float ref_scale[kRows];
+  __shared__ uint8_t has_far[2][kRows];
+  constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
+  constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = (int)blockIdx.x / sh.slices, slice = (int)blockIdx.x % sh.slices;
+  const int s0 = (int)((unsigned)sh.steps * (unsigned)slice / (unsigned)sh.slices);
+  const int s1 = (int)((unsigned)sh.steps * (slice + 1u) / (unsigned)sh.slices);
+  const int row0 = tile * kRows, token0 = (int)blockIdx.y * 128;
+  const int cols = (int)(a.T - token0 < 128 ? a.T - token0 : 128);
+  const uint32_t x_bytes = (uint32_t)sh.tokens * sk * 2, slot_bytes = kRows * kCodeBytes + x_bytes;
+  auto full = [&](int s) { return smem_u32(&bars[s]); };
+  auto empty = [&](int s) { return smem_u32(&bars[kMaxStages + s]); };
+  auto a_full = [&](int b) { return smem_u32(&bars[2 * kMaxStages + b]); };
+  auto a_empty = [&](int b) { return smem_u32(&bars[2 * kMaxStages + 2 + b]); };
+  const uint32_t done = smem_u32(&bars[2 * kMaxStages + 4]);
+
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(a_full(b), kDecodeWarps);
+      mbar_init(a_empty(b), 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  if (warp == kDecodeWarps) {
+    tmem_alloc<1>(smem_u32(&tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tmem_a = tmem + 128;  // sums, then two decoded steps
+
+  if (warp == kDecodeWarps + 1) {
+    // ---- copies: codes at once, x when the first kernel has laid it out
+    if (elect_one()) {
+      const uint64_t once = l2_policy_evict_normal(), keep = l2_policy_evict_last();
+      auto ask_codes = [&](int step, int stage) {
+        mbar_arrive_expect_tx(full(stage), slot_bytes);
+        tma_load_2d(ring + stage * slot_bytes, &map_w, step * kCodeBytes, row0, full(stage), once);
+      };
+      auto ask_x = [&](int step, int stage) {
+        const uint32_t at = ring + stage * slot_bytes + kRows * kCodeBytes;
+        for (int i = 0; i < sk / 64; ++i)
+          tma_load_2d(at + i * sh.tokens * 128, &map_x, step * sk + i * 64, token0, full(stage), keep);
+      };
+      const int first = s1 - s0 < sh.stages ? s1 - s0 : sh.stages;
+      for (int i = 0; i < first; ++i) ask_codes(s0 + i, i);
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < first; ++i) ask_x(s0 + i, i);
+      int stage = 0;
+      uint32_t round = 0;
+      int asked = first;
+      for (int i = first; i < s1 - s0; ++i) {
+        if (!mbar_wait(empty(stage), round, &aborted, a.err, ERRW_TIMEOUT_PRODUCER, a.wait_ns)) break;
+        ask_codes(s0 + i, stage);
+        ask_x(s0 + i, stage);
+        ++asked;
+        if (++stage == sh.stages) {
+          stage = 0;
+          round ^= 1u;
+        }
+      }
+      // every copy lands before the CTA ends
+      int none = 0;
+      for (int i = asked > sh.stages ? asked - sh.stages : 0; i < asked; ++i)
+        mbar_wait(full(i % sh.stages), (uint32_t)(i / sh.stages) & 1u, &none, nullptr, 0, a.wait_ns);
+    }
+    __syncwarp();
+  } else if (warp == kDecodeWarps) {
+    // ---- products
+    const uint32_t idesc = encode_idesc(KIND_F16, 0, 0, 128, sh.tokens, 0, 0);
+    const uint32_t on = elect_one() ? 1u : 0u;
+    int stage = 0;
+    uint32_t round = 0;
+    for (int i = 0; i < s1 - s0; ++i) {
+      const int b = i & 1;
+      bool ok = mbar_wait(full(stage), round, &aborted, a.err, ERRW_TIMEOUT_MMA, a.wait_ns);
+      ok = ok && mbar_wait(a_full(b), (uint32_t)(i >> 1) & 1u, &aborted, a.err, ERRW_TIMEOUT_MMA, a.wait_ns);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t x = ring + stage * slot_bytes + kRows * kCodeBytes;
+#pragma unroll
+      for (int k = 0; k < sk / 16; ++k) {
+        const uint64_t bd = encode_smem_desc(x + k / 4 * sh.tokens * 128 + k % 4 * 32, 16, 1024, SWZ_128B);
+        mma_ts<1, KIND_F16>(tmem, tmem_a + b * a_cols + 8 * k, bd, idesc, (i | k) != 0 ? 1u : 0u, on);
+      }
+      tc_commit<1>(a_empty(b), on);
+      tc_commit<1>(empty(stage), on);
+      __syncwarp();
+      if (++stage == sh.stages) {
+        stage = 0;
+        round ^= 1u;
+      }
+    }
+    tc_commit<1>(done, on);
+    // nothing of this warp is in flight when tensor memory is given back
+    int none = 0;
+    if (!mbar_wait(done, 0, &none, nullptr, 0, a.wait_ns) && on) {
+      aborted = 1;
+      if (a.err) atomicOr(a.err, ERRW_TIMEOUT_MMA);
+    }
+    __syncwarp();
+  } else {
+    // ---- decoding: row `r`, half `half` of each step
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int row = row0 + r < (int)a.N ? row0 + r : (int)a.N - 1;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int scales = (int)a.kp / bf_block(FMT);             // of a row
+    constexpr int per_step = sk / bf_block(FMT);
+    const uint8_t* sf = a.sf + (int64_t)row * scales;
+    uint32_t ref = 0;
+    float* far = nullptr;
+    if constexpr (FMT != BF_NVFP4) {
+      const int end = s1 * per_step < scales ? s1 * per_step : scales;
+      uint32_t top = 0;
+      int i = s0 * per_step;
+      if (((reinterpret_cast<uintptr_t>(sf) | (uintptr_t)i) & 3) == 0)
+#pragma unroll 8
+        for (; i + 4 <= end; i += 4) top = __vmaxu4(top, __ldg(reinterpret_cast<const uint32_t*>(sf + i)));
+      top = __vmaxu4(top, top >> 16);
+      ref = max(top & 0xFFu, (top >> 8) & 0xFFu);
+      for (; i < end; ++i) ref = max(ref, (uint32_t)__ldg(sf + i));
+      if (ref == 255u) {  // a NaN scale says nothing of the others
+        ref = 0;
+        for (i = s0 * per_step; i < end; ++i) {
+          const uint32_t s = __ldg(sf + i);
+          ref = s > ref && s != 255u ? s : ref;
+        }
+      }
+      if (half == 0) ref_scale[r] = e8m0_value(ref);
+      has_far[half][r] = 0;
+      far = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + half) * kRows + r) * 128;
+    }
+    int stage = 0;
+    uint32_t round = 0;
+    bool any_far = false;
+    uint2 sc = load_scales<FMT>(sf, s0 * per_step + half * (per_step / 2), scales, sh.words);
+    for (int i = 0; i < s1 - s0; ++i) {
+      const int b = i & 1;
+      const uint2 now = sc;
+      if (i + 1 < s1 - s0)
+        sc = load_scales<FMT>(sf, (s0 + i + 1) * per_step + half * (per_step / 2), scales, sh.words);
+      bool ok = mbar_wait(full(stage), round, &aborted, a.err, ERRW_TIMEOUT_OTHER, a.wait_ns);
+      ok = ok && (i < 2 || mbar_wait(a_empty(b), (uint32_t)((i >> 1) - 1) & 1u, &aborted, a.err,
+                                     ERRW_TIMEOUT_OTHER, a.wait_ns));
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t slot = ring + stage * slot_bytes;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int piece = half * 4 + p;
+        uint32_t c[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                     : "r"(slot + r * kCodeBytes + ((piece ^ (r & 7)) << 4))
+                     : "memory");
+        // multipliers of the piece's halves
+        uint32_t m[2];
+        if constexpr (FMT == BF_NVFP4) {
+          const uint32_t word = p < 2 ? now.x : now.y;
+          uint32_t h;
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(word >> (16 * (p & 1)))));
+          m[0] = __byte_perm(h, 0, 0x1010);
+          m[1] = __byte_perm(h, 0, 0x3232);
+        } else {
+          const uint32_t s = (now.x >> (8 * (FMT == BF_MXF8 ? p / 2 : p))) & 0xFFu;
+          const int d = (int)s - (int)ref;
+          m[0] = s == 255u ? 0x7E007E00u : (uint32_t)(d + 15) * 0x04000400u;
+          if (d < -14) {
+            m[0] = 0u;
+            if ((c[0] | c[1] | c[2] | c[3]) & (FMT == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) {
+              if (!any_far) {
+                any_far = true;
+                has_far[half][r] = 1;
+                for (int t = 0; t < sh.tokens; ++t) far[t] = 0.0f;
+              }
+              far_block<FMT>(c, s, slot + kRows * kCodeBytes, sh.tokens, piece * elems, far);
+            }
+          }
+          m[1] = m[0];
+        }
+        uint32_t f[elems / 2];
+        if constexpr (FMT == BF_MXF8) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f[k]) : "h"((uint16_t)(c[k >> 1] >> (16 * (k & 1)))));
+            f[k] = mul_h2(f[k], m[0]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t q[4];
+            e2m1x8_pairs(c[k], q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[4 * k + j] = mul_h2(q[j], m[k >> 1]);
+          }
+        }
+        const uint32_t to = tmem_a + b * a_cols + lanes + piece * (elems / 2);
+        __syncwarp();  // lanes with far blocks took longer
+        if constexpr (FMT == BF_MXF8) {
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(to),
+                       "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]), "r"(f[4]), "r"(f[5]), "r"(f[6]), "r"(f[7])
+                       : "memory");
+        } else {
+          tmem_st_32x32b_x16(to, f);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_full(b));
+      if (++stage == sh.stages) {
+        stage = 0;
+        round ^= 1u;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();  // the products are done (their warp waited for them)
+  tc_fence_after();
+  const int n = (int)a.N;
+  const int64_t at = (int64_t)blockIdx.y * sh.row_tiles + tile;
+  float* mine = part + (at * sh.slices + slice) * ((int64_t)sh.tokens * kRows);
+  if (warp < kDecodeWarps && !aborted) {
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float scale = FMT == BF_NVFP4 ? 1.0f : ref_scale[r];
+    const bool far0 = FMT != BF_NVFP4 && has_far[0][r], far1 = FMT != BF_NVFP4 && has_far[1][r];
+    const float* f0 = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2) * kRows + r) * 128;
+    for (int c = half * 16; c < sh.tokens; c += 32) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(tmem + lanes + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = c + i;
+        if (t >= cols) break;
+        const float d = __uint_as_float(v[i]);
+        float sum = FMT == BF_NVFP4 || d == 0.0f ? d : d * scale;
+        if (far0) sum += __ldcg(f0 + t);
+        if (far1) sum += __ldcg(f0 + kRows * 128 + t);
+        if (sh.slices > 1)
+          __stcg(mine + t * kRows + r, sum);
+        else if (row0 + r < n)
+          static_cast<T*>(a.out)[(int64_t)(token0 + t) * a.ld_out + row0 + r] =
+              from_f32<T>(a.alpha * (sum * __ldcg(xs + token0 + t)));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kDecodeWarps) tmem_dealloc<1>(tmem, 512);
+  if (sh.slices == 1) return;
+  // the CTA that arrives last adds the slices, always in the same order
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atomicAdd(a.count + at, 1u) == (uint32_t)sh.slices - 1u;
+    if (last) a.count[at] = 0u;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float* all = part + at * sh.slices * ((int64_t)sh.tokens * kRows);
+  for (int e = threadIdx.x; e < cols * kRows; e += kThreads) {
+    const int t = e / kRows, r = e % kRows;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < sh.slices; ++k) sum += __ldcg(all + (int64_t)k * sh.tokens * kRows + e);
+    if (row0 + r < n)
+      static_cast<T*>(a.out)[(int64_t)(token0 + t) * a.ld_out + row0 + r] =
+          from_f32<T>(a.alpha * (sum * __ldcg(xs + token0 + t)));
+  }
+}
+
+TileShape tile_shape(int fmt, const FewLinearArgs& a, int sm_count) {
+  TileShape s;
+  const int64_t t = a.T < 128 ? a.T : 128;
+  s.tokens = (int)((t + 15) / 16 * 16);
+  s.z = (int)((a.T + 127) / 128);
+  s.steps = (int)((a.kp + step_k(fmt) - 1) / step_k(fmt));
+  s.row_tiles = (int)((a.N + kRows - 1) / kRows);
+  const int scales = step_k(fmt) / 2 / bf_block(fmt);  // a thread's of a step
+  s.words = a.kp / bf_block(fmt) % scales == 0 && (reinterpret_cast<uintptr_t>(a.sf) % scales) == 0;
+  // one CTA an SM; K is cut as far as there are SMs left and each CTA keeps two steps
+  int n = sm_count / (s.row_tiles * s.z);
+  n = n < s.steps / 2 ? n : s.steps / 2;
+  s.slices = n < 1 ? 1 : n;
+  const int slot = kRows * kCodeBytes + s.tokens * step_k(fmt) * 2;
+  s.stages = (220 * 1024) / slot < kMaxStages ? (220 * 1024) / slot : kMaxStages;
+  s.smem = s.stages * slot + 1024;
+  // tensor memory is taken whole: one CTA an SM
+  if (s.smem < 120 * 1024) s.smem = 120 * 1024;
+  return s;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+struct TileWs {
+  size_t x16, xs, far, part, total;
+};
+
+TileWs tile_ws(int fmt, const FewLinearArgs& a, const TileShape& s) {
+  TileWs w;
+  w.x16 = 0;
+  w.xs = up256((size_t)a.T * s.steps * step_k(fmt) * 2);
+  w.far = w.xs + up256((size_t)a.T * sizeof(float));
+  const size_t ctas = (size_t)s.row_tiles * s.slices * s.z;
+  w.part = w.far + (fmt == BF_NVFP4 ? 0 : ctas * 2 * kRows * 128 * sizeof(float));
+  w.total = w.part + (s.slices > 1 ? ctas * s.tokens * kRows * sizeof(float) : 0);
+  return w;
+}
+
+template <typename T, int FMT>
+cudaError_t tiles_launch(const FewLinearArgs& a, const TileShape& sh, const CUtensorMap& mw,
+                         const CUtensorMap& mx, const TileWs& w, cudaStream_t s) {
+  char* ws = static_cast<char*>(a.ws);
+  float* xs = reinterpret_cast<float*>(ws + w.xs);
+  tiles_prepare_kernel<T><<<(unsigned)a.T, 512, 0, s>>>(a, (int64_t)sh.steps * step_k(FMT),
+                                                        reinterpret_cast<__half*>(ws + w.x16), xs);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  static std::atomic<int> seen[16];
+  e = allow_smem(few_tiles_kernel<T, FMT>, sh.smem, seen);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(sh.row_tiles * sh.slices), (unsigned)sh.z);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)sh.smem;
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, few_tiles_kernel<T, FMT>, mw, mx, a, sh, static_cast<const float*>(xs),
+                            reinterpret_cast<float*>(ws + w.part), reinterpret_cast<float*>(ws + w.far));
+}
+
+}  // namespace
+
+size_t few_tiles_ws_bytes(int fmt, const FewLinearArgs& a, int sm_count) {
+  return tile_ws(fmt, a, tile_shape(fmt, a, sm_count)).total;
+}
+
+size_t few_tiles_counters(int fmt, const FewLinearArgs& a, int sm_count) {
+  const TileShape s = tile_shape(fmt, a, sm_count);
+  return s.slices > 1 ? (size_t)s.row_tiles * s.z : 0;
+}
+
+void few_tiles_maps(int fmt, const FewLinearArgs& a, int sm_count, FewTilesMaps* m) {
+  const TileShape s = tile_shape(fmt, a, sm_count);
+  m->w_row_bytes = (uint64_t)(a.kp * bf_bits(fmt) / 8);
+  m->w_box_bytes = kCodeBytes;
+  m->w_box_rows = kRows;
+  m->x_cols = (uint64_t)s.steps * step_k(fmt);
+  m->x_box_cols = 64;
+  m->x_box_rows = (uint32_t)s.tokens;
+}
+
+cudaError_t launch_few_tiles(int fmt, int type, const FewLinearArgs& a, const CUtensorMap& map_w,
+                             const CUtensorMap& map_x, int sm_count, cudaStream_t s) {
+  const TileShape sh = tile_shape(fmt, a, sm_count);
+  const TileWs w = tile_ws(fmt, a, sh);
+  if (type == B2G_BF16) {
+    if (fmt == BF_NVFP4) return tiles_launch<__nv_bfloat16, BF_NVFP4>(a, sh, map_w, map_x, w, s);
+    if (fmt == BF_MXF4) return tiles_launch<__nv_bfloat16, BF_MXF4>(a, sh, map_w, map_x, w, s);
+    return tiles_launch<__nv_bfloat16, BF_MXF8>(a, sh, map_w, map_x, w, s);
+  }
+  if (fmt == BF_NVFP4) return tiles_launch<__half, BF_NVFP4>(a, sh, map_w, map_x, w, s);
+  if (fmt == BF_MXF4) return tiles_launch<__half, BF_MXF4>(a, sh, map_w, map_x, w, s);
+  return tiles_launch<__half, BF_MXF8>(a, sh, map_w, map_x, w, s);
+}
+
+}  // namespace b2g

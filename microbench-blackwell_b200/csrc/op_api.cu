@@ -64,6 +64,25 @@ b2g_status grow(b2g_handle* h, size_t bytes, size_t words, cudaStream_t s) {
   return B2G_OK;
 }
 
+// 128-byte swizzled map of a row-major matrix whose rows follow one another.
+b2g_status tensor_map(b2g_handle* h, CUtensorMap* map, CUtensorMapDataType type, int elem,
+                      const void* base, uint64_t cols, uint64_t rows, uint32_t box_cols,
+                      uint32_t box_rows) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * (uint64_t)elem};
+  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+  const CUresult r = h->encode_tiled(map, type, 2, const_cast<void*>(base), dims, strides, box, one,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(h, B2G_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) dims=%llu x %llu", (int)r,
+                (unsigned long long)cols, (unsigned long long)rows);
+  return B2G_OK;
+}
+
+// b2g_linear: from this many tokens on the tensor-core form.
+constexpr int kTilesFrom = 9;
+
 }  // namespace
 
 extern "C" {
@@ -348,12 +367,30 @@ b2g_status b2g_linear(b2g_handle* h, const b2g_linear_desc* d, void* stream) {
   a.x_vec = rows_aligned(d->x, d->ld_x, 2, 16);
   DeviceGuard g(h->device);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const b2g_status st = grow(h, few_linear_ws_bytes(fmt, a, h->sm_count),
-                             few_linear_counters(fmt, a, h->sm_count), s);
+  a.err = h->d_err;
+  a.wait_ns = h->wait_ns;
+  const bool tiles = d->T >= kTilesFrom;
+  const b2g_status st = tiles ? grow(h, few_tiles_ws_bytes(fmt, a, h->sm_count),
+                                     few_tiles_counters(fmt, a, h->sm_count), s)
+                              : grow(h, few_linear_ws_bytes(fmt, a, h->sm_count),
+                                     few_linear_counters(fmt, a, h->sm_count), s);
   if (st != B2G_OK) return st;
   a.ws = h->op_ws;
   a.count = h->op_count;
-  B2G_CUDA(h, launch_few_linear(fmt, d->type, a, h->sm_count, s));
+  if (!tiles) {
+    B2G_CUDA(h, launch_few_linear(fmt, d->type, a, h->sm_count, s));
+    return B2G_OK;
+  }
+  FewTilesMaps m;
+  few_tiles_maps(fmt, a, h->sm_count, &m);
+  CUtensorMap map_w, map_x;
+  b2g_status mt = tensor_map(h, &map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, d->w, m.w_row_bytes,
+                             (uint64_t)d->N, m.w_box_bytes, m.w_box_rows);
+  if (mt != B2G_OK) return mt;
+  mt = tensor_map(h, &map_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.ws, m.x_cols, (uint64_t)d->T,
+                  m.x_box_cols, m.x_box_rows);
+  if (mt != B2G_OK) return mt;
+  B2G_CUDA(h, launch_few_tiles(fmt, d->type, a, map_w, map_x, h->sm_count, s));
   return B2G_OK;
 }
 

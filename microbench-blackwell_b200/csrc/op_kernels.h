@@ -1,6 +1,7 @@
 // op_kernels.h -- internal interface between the C entries of the operators around the
 // linear layer (op_api.cu) and their kernels.  Not part of the public ABI.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -84,11 +85,25 @@ struct FewLinearArgs {
   int64_t ld_out;
   float alpha;
   int x_vec;  // every row of `x` starts on 16 bytes
-  void* ws;   // few_linear_ws_bytes() bytes
-  uint32_t* count;  // few_linear_counters() words, zero before and after
+  void* ws;   // few_linear_ws_bytes() or few_tiles_ws_bytes() bytes
+  uint32_t* count;  // ..._counters() words, zero before and after
+  uint32_t* err;    // the handle's error word
+  uint64_t wait_ns; // limit of bounded waits (0: default)
 };
 size_t few_linear_ws_bytes(int fmt, const FewLinearArgs& a, int sm_count);
 size_t few_linear_counters(int fmt, const FewLinearArgs& a, int sm_count);
+// Its tensor-core form (few_tiles.cu): map_w over the codes' bytes [N][row bytes], map_x over
+// fp16 [T][x_cols] at the start of the workspace, boxes as few_tiles_maps() says, both with
+// the 128-byte swizzle.
+struct FewTilesMaps {
+  uint64_t w_row_bytes, x_cols;
+  uint32_t w_box_bytes, w_box_rows, x_box_cols, x_box_rows;
+};
+void few_tiles_maps(int fmt, const FewLinearArgs& a, int sm_count, FewTilesMaps* m);
+size_t few_tiles_ws_bytes(int fmt, const FewLinearArgs& a, int sm_count);
+size_t few_tiles_counters(int fmt, const FewLinearArgs& a, int sm_count);
+cudaError_t launch_few_tiles(int fmt, int type, const FewLinearArgs& a, const CUtensorMap& map_w,
+                             const CUtensorMap& map_x, int sm_count, cudaStream_t s);
 cudaError_t launch_few_linear(int fmt, int type, const FewLinearArgs& a, int sm_count,
                               cudaStream_t s);
 
