@@ -2,7 +2,7 @@
 // tensor-core form of b2g_linear (few_linear.cu has the form for a handful).
 //
 // The weights are the 128-row operand A of tcgen05.mma kind::f16, taken from tensor memory:
-// eight warps decode codes to fp16 (exact, as in few_linear.cu) and write them there, a row
+// sixteen warps decode codes to fp16 (exact, as in few_linear.cu) and write them there, a row
 // a thread, so that decoded weights never pass through shared memory.  x, laid out as fp16
 // by a first kernel, is operand B, up to 128 tokens of it; sums stay in tensor memory until
 // the end.  A decoded weight then serves all tokens for one instruction's issue, and what
@@ -20,10 +20,13 @@ namespace b2g {
 namespace {
 
 constexpr int kRows = 128;            // weight rows of a CTA
-constexpr int kDecodeWarps = 8;       // four for each half of a step
+constexpr int kParts = 4;             // of a step, each decoded by four warps
+constexpr int kDecodeWarps = 4 * kParts;
+constexpr int kPieces = 8 / kParts;   // 16-byte pieces of a row in a part
 constexpr int kThreads = (kDecodeWarps + 2) * 32;
 constexpr int kCodeBytes = 128;       // of a row in a step
 constexpr int kMaxStages = 4;
+constexpr int kScaleBytes = 2048;     // of a ring slot: 16, 8 or 4 bytes a row
 
 __host__ __device__ constexpr int step_k(int fmt) { return kCodeBytes * 8 / bf_bits(fmt); }
 
@@ -33,7 +36,7 @@ struct TileShape {
   int slices;    // of K, one a CTA
   int row_tiles, z;
   int stages;
-  int words;     // a thread's scales of a half step are one aligned word
+  int words;     // a row's scales of a step are one aligned word, copied into the ring
   int smem;
 };
 
@@ -106,77 +109,79 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A thread's scale bytes of half a step: NVFP4 8, MXFP4 4, MXFP8 2, in the low bytes.
+// A thread's scale bytes of a part: NVFP4 4, MXFP4 2, MXFP8 1; zeros past the row's end.
 template <int FMT>
-__device__ __forceinline__ uint2 load_scales(const uint8_t* row, int first, int count, bool words) {
-  constexpr int n = step_k(FMT) / 2 / bf_block(FMT);
-  uint2 s = make_uint2(0u, 0u);
-  if (words) {  // whole and aligned, or past the row's end
-    if (first < count) {
-      if constexpr (n == 8)
-        s = __ldg(reinterpret_cast<const uint2*>(row + first));
-      else if constexpr (n == 4)
-        s.x = __ldg(reinterpret_cast<const uint32_t*>(row + first));
-      else
-        s.x = __ldg(reinterpret_cast<const uint16_t*>(row + first));
-    }
-  } else {
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* row, int first, int count) {
+  constexpr int n = step_k(FMT) / kParts / bf_block(FMT);
+  uint32_t s = 0u;
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const uint32_t b = first + i < count ? __ldg(row + first + i) : 0u;
-      if (i < 4)
-        s.x |= b << (8 * i);
-      else
-        s.y |= b << (8 * (i - 4));
-    }
-  }
+  for (int i = 0; i < n; ++i) s |= (first + i < count ? (uint32_t)__ldg(row + first + i) : 0u) << (8 * i);
   return s;
 }
 
-// Rows of the weights' scales within a CTA's K slice share one power of two (MX), the
-// largest scale of the row there: 2^(s - ref) times an element is exact in fp16 down to
-// 2^-14.  A block below that (and not all zeros) is left out of the tensor product and
-// multiplied in fp32 by its own thread, into far[token] of the row.
+// MX: the scales of a row within a CTA's K slice are taken relative to one of them, the
+// largest of a few samples: 2^(s - ref) times an element is exact and finite in fp16 for s
+// - ref from -14 to 13 (e2m1) or 7 (e4m3).  Blocks outside (and not all zeros) are left out
+// of the tensor product.
 template <int FMT>
-__device__ __noinline__ void far_block(const uint32_t (&codes)[4], uint32_t scale, uint32_t x_stage,
-                                       int tokens, int k, float* far) {
-  constexpr int elems = 128 / bf_bits(FMT);
-  const float s = e8m0_value(scale);
-  for (int t = 0; t < tokens; ++t) {
-    float dot = 0.0f;
-    for (int i = 0; i < elems; ++i) {
-      const int kk = k + i, byte = kk % 64 * 2;
-      const uint32_t at = x_stage + (kk / 64 * tokens + t) * 128 + (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15);
-      uint16_t h;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
-      const uint32_t word = codes[i * bf_bits(FMT) / 32] >> (i * bf_bits(FMT) % 32);
-      float c;
-      if constexpr (FMT == BF_MXF8) {
-        c = e4m3_pair(word & 0xFFu).x;
-      } else {
-        uint32_t p[4];
-        e2m1x8_pairs(word & 15u, p);
-        c = __half2float(__ushort_as_half((unsigned short)(p[0] & 0xFFFFu)));
+__device__ __forceinline__ bool far_scale(uint32_t s, uint32_t ref) {
+  const int d = (int)s - (int)ref;
+  return s != 255u && (d < -14 || d > (FMT == BF_MXF8 ? 7 : 13));
+}
+
+__device__ __forceinline__ bool any_code(int fmt, const uint4& c) {
+  return ((c.x | c.y | c.z | c.w) & (fmt == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) != 0u;
+}
+
+// Their products, in fp32 and from global memory, by the thread that decodes them: the part
+// pt of every step of one row, into far[token].  x16: the CTA's first token.
+template <int FMT>
+__device__ __noinline__ void far_blocks(const FewLinearArgs& a, const __half* x16, int64_t kq, int row,
+                                        int s0, int s1, int pt, uint32_t ref, int cols, float* far) {
+  constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
+  for (int t = 0; t < cols; ++t) far[t] = 0.0f;
+  const int scales = (int)a.kp / bf_block(FMT);
+  for (int step = s0; step < s1; ++step)
+    for (int p = 0; p < kPieces; ++p) {
+      const int k0 = step * sk + (pt * kPieces + p) * elems;
+      if (k0 >= a.kp) continue;
+      const uint32_t s = __ldg(a.sf + (int64_t)row * scales + k0 / bf_block(FMT));
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(a.w + ((int64_t)row * a.kp + k0) * bf_bits(FMT) / 8));
+      if (!far_scale<FMT>(s, ref) || !any_code(FMT, c)) continue;
+      for (int t = 0; t < cols; ++t) {
+        float dot = 0.0f;
+        for (int i = 0; i < elems; ++i) {
+          const int at = i * bf_bits(FMT) / 32;
+          const uint32_t word = (at == 0 ? c.x : at == 1 ? c.y : at == 2 ? c.z : c.w) >> (i * bf_bits(FMT) % 32);
+          float v;
+          if constexpr (FMT == BF_MXF8) {
+            v = e4m3_pair(word & 0xFFu).x;
+          } else {
+            uint32_t q[4];
+            e2m1x8_pairs(word & 15u, q);
+            v = __half2float(__ushort_as_half((unsigned short)(q[0] & 0xFFFFu)));
+          }
+          dot = fmaf(v, __half2float(x16[t * kq + k0 + i]), dot);
+        }
+        far[t] = fmaf(e8m0_value(s), dot, far[t]);
       }
-      dot = fmaf(c, __half2float(__ushort_as_half(h)), dot);
     }
-    far[t] = fmaf(s, dot, far[t]);
-  }
 }
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
 few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                 const FewLinearArgs a, const TileShape sh, const float* xs, float* part, float* far_ws) {
+                 const FewLinearArgs a, const TileShape sh, const __half* x16, const float* xs,
+                 float* part, float* far_ws) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  // ring slots (codes, then x) start on 1024 bytes
+  // ring slots (codes, x, scales) start on 1024 bytes
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4 + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
   __shared__ bool last;
   __shared__ float ref_scale[kRows];
-  __shared__ uint8_t has_far[2][kRows];
+  __shared__ uint8_t has_far[kParts][kRows];
   constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
   constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -185,7 +190,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const int s1 = (int)((unsigned)sh.steps * (slice + 1u) / (unsigned)sh.slices);
   const int row0 = tile * kRows, token0 = (int)blockIdx.y * 128;
   const int cols = (int)(a.T - token0 < 128 ? a.T - token0 : 128);
-  const uint32_t x_bytes = (uint32_t)sh.tokens * sk * 2, slot_bytes = kRows * kCodeBytes + x_bytes;
+  const uint32_t x_bytes = (uint32_t)sh.tokens * sk * 2, slot_bytes = kRows * kCodeBytes + x_bytes + kScaleBytes;
   auto full = [&](int s) { return smem_u32(&bars[s]); };
   auto empty = [&](int s) { return smem_u32(&bars[kMaxStages + s]); };
   auto a_full = [&](int b) { return smem_u32(&bars[2 * kMaxStages + b]); };
@@ -195,7 +200,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   if (threadIdx.x == 0) {
     aborted = 0;
     for (int s = 0; s < kMaxStages; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), 1 + 32);  // the copies' byte count, and a lane's scales each
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -215,40 +220,63 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const uint32_t tmem = tmem_slot, tmem_a = tmem + 128;  // sums, then two decoded steps
 
   if (warp == kDecodeWarps + 1) {
-    // ---- copies: codes at once, x when the first kernel has laid it out
-    if (elect_one()) {
-      const uint64_t once = l2_policy_evict_normal(), keep = l2_policy_evict_last();
-      auto ask_codes = [&](int step, int stage) {
-        mbar_arrive_expect_tx(full(stage), slot_bytes);
+    // ---- copies: codes and scales at once, x when the first kernel has laid it out
+    const bool one = elect_one();
+    const uint64_t once = l2_policy_evict_normal(), keep = l2_policy_evict_last();
+    constexpr int n = sk / bf_block(FMT);  // scale bytes of a row in a step
+    const int scales = (int)a.kp / bf_block(FMT);
+    auto ask_codes = [&](int step, int stage) {
+      if (one) {
+        mbar_arrive_expect_tx(full(stage), kRows * kCodeBytes + x_bytes);
         tma_load_2d(ring + stage * slot_bytes, &map_w, step * kCodeBytes, row0, full(stage), once);
-      };
-      auto ask_x = [&](int step, int stage) {
-        const uint32_t at = ring + stage * slot_bytes + kRows * kCodeBytes;
-        for (int i = 0; i < sk / 64; ++i)
-          tma_load_2d(at + i * sh.tokens * 128, &map_x, step * sk + i * 64, token0, full(stage), keep);
-      };
-      const int first = s1 - s0 < sh.stages ? s1 - s0 : sh.stages;
-      for (int i = 0; i < first; ++i) ask_codes(s0 + i, i);
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      for (int i = 0; i < first; ++i) ask_x(s0 + i, i);
-      int stage = 0;
-      uint32_t round = 0;
-      int asked = first;
-      for (int i = first; i < s1 - s0; ++i) {
-        if (!mbar_wait(empty(stage), round, &aborted, a.err, ERRW_TIMEOUT_PRODUCER, a.wait_ns)) break;
-        ask_codes(s0 + i, stage);
-        ask_x(s0 + i, stage);
-        ++asked;
-        if (++stage == sh.stages) {
-          stage = 0;
-          round ^= 1u;
+      }
+      if (sh.words) {
+        const uint32_t to = ring + stage * slot_bytes + kRows * kCodeBytes + x_bytes;
+        const bool on = step * n < scales;
+#pragma unroll
+        for (int k = 0; k < kRows / 32; ++k) {
+          const int r = k * 32 + lane, row = row0 + r < (int)a.N ? row0 + r : (int)a.N - 1;
+          const uint8_t* src = a.sf + (int64_t)row * scales + (on ? step * n : 0);
+          if constexpr (n == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * n), "l"(src),
+                         "r"(on ? n : 0)
+                         : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to + r * n), "l"(src),
+                         "n"(n), "r"(on ? n : 0)
+                         : "memory");
         }
       }
-      // every copy lands before the CTA ends
-      int none = 0;
-      for (int i = asked > sh.stages ? asked - sh.stages : 0; i < asked; ++i)
-        mbar_wait(full(i % sh.stages), (uint32_t)(i / sh.stages) & 1u, &none, nullptr, 0, a.wait_ns);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(full(stage)) : "memory");
+    };
+    auto ask_x = [&](int step, int stage) {
+      const uint32_t at = ring + stage * slot_bytes + kRows * kCodeBytes;
+      if (one)
+        for (int i = 0; i < sk / 64; ++i)
+          tma_load_2d(at + i * sh.tokens * 128, &map_x, step * sk + i * 64, token0, full(stage), keep);
+    };
+    const int first = s1 - s0 < sh.stages ? s1 - s0 : sh.stages;
+    for (int i = 0; i < first; ++i) ask_codes(s0 + i, i);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = 0; i < first; ++i) ask_x(s0 + i, i);
+    int stage = 0;
+    uint32_t round = 0;
+    int asked = first;
+    for (int i = first; i < s1 - s0; ++i) {
+      const bool ok = mbar_wait(empty(stage), round, &aborted, a.err, ERRW_TIMEOUT_PRODUCER, a.wait_ns);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      ask_codes(s0 + i, stage);
+      ask_x(s0 + i, stage);
+      ++asked;
+      if (++stage == sh.stages) {
+        stage = 0;
+        round ^= 1u;
+      }
     }
+    // every copy lands before the CTA ends
+    int none = 0;
+    for (int i = asked > sh.stages ? asked - sh.stages : 0; i < asked; ++i)
+      mbar_wait(full(i % sh.stages), (uint32_t)(i / sh.stages) & 1u, &none, nullptr, 0, a.wait_ns);
     __syncwarp();
   } else if (warp == kDecodeWarps) {
     // ---- products
@@ -286,8 +314,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     }
     __syncwarp();
   } else {
-    // ---- decoding: row `r`, half `half` of each step
-    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    // ---- decoding: row `r`, part `pt` of each step
+    const int pt = warp >> 2, r = (warp & 3) * 32 + lane;
     const int row = row0 + r < (int)a.N ? row0 + r : (int)a.N - 1;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int scales = (int)a.kp / bf_block(FMT);             // of a row
@@ -296,35 +324,25 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     uint32_t ref = 0;
     float* far = nullptr;
     if constexpr (FMT != BF_NVFP4) {
-      const int end = s1 * per_step < scales ? s1 * per_step : scales;
-      uint32_t top = 0;
-      int i = s0 * per_step;
-      if (((reinterpret_cast<uintptr_t>(sf) | (uintptr_t)i) & 3) == 0)
-#pragma unroll 8
-        for (; i + 4 <= end; i += 4) top = __vmaxu4(top, __ldg(reinterpret_cast<const uint32_t*>(sf + i)));
-      top = __vmaxu4(top, top >> 16);
-      ref = max(top & 0xFFu, (top >> 8) & 0xFFu);
-      for (; i < end; ++i) ref = max(ref, (uint32_t)__ldg(sf + i));
-      if (ref == 255u) {  // a NaN scale says nothing of the others
-        ref = 0;
-        for (i = s0 * per_step; i < end; ++i) {
-          const uint32_t s = __ldg(sf + i);
-          ref = s > ref && s != 255u ? s : ref;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int step = s0 + (s1 - s0) * q / 8;
+        const uint32_t w = load_scales<FMT>(sf, step * per_step, scales);
+#pragma unroll
+        for (int i = 0; i < per_step / kParts; ++i) {
+          const uint32_t s = (w >> (8 * i)) & 0xFFu;
+          ref = s > ref && s != 255u ? s : ref;  // a NaN scale says nothing of the others
         }
       }
-      if (half == 0) ref_scale[r] = e8m0_value(ref);
-      has_far[half][r] = 0;
-      far = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + half) * kRows + r) * 128;
+      if (pt == 0) ref_scale[r] = e8m0_value(ref);
+      far = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kParts + pt) * kRows + r) * 128;
     }
     int stage = 0;
     uint32_t round = 0;
     bool any_far = false;
-    uint2 sc = load_scales<FMT>(sf, s0 * per_step + half * (per_step / 2), scales, sh.words);
+    constexpr int mine_n = per_step / kParts;  // scale bytes of a part
     for (int i = 0; i < s1 - s0; ++i) {
       const int b = i & 1;
-      const uint2 now = sc;
-      if (i + 1 < s1 - s0)
-        sc = load_scales<FMT>(sf, (s0 + i + 1) * per_step + half * (per_step / 2), scales, sh.words);
       bool ok = mbar_wait(full(stage), round, &aborted, a.err, ERRW_TIMEOUT_OTHER, a.wait_ns);
       ok = ok && (i < 2 || mbar_wait(a_empty(b), (uint32_t)((i >> 1) - 1) & 1u, &aborted, a.err,
                                      ERRW_TIMEOUT_OTHER, a.wait_ns));
@@ -332,9 +350,24 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const uint32_t slot = ring + stage * slot_bytes;
+      uint32_t now;
+      if (sh.words) {
+        const uint32_t at = slot + kRows * kCodeBytes + x_bytes + r * per_step + pt * mine_n;
+        if constexpr (mine_n == 4) {
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
+        } else if constexpr (mine_n == 2) {
+          uint16_t h;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
+          now = h;
+        } else {
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
+        }
+      } else {
+        now = load_scales<FMT>(sf, (s0 + i) * per_step + pt * mine_n, scales);
+      }
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int piece = half * 4 + p;
+      for (int p = 0; p < kPieces; ++p) {
+        const int piece = pt * kPieces + p;
         uint32_t c[4];
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
@@ -343,25 +376,17 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         // multipliers of the piece's halves
         uint32_t m[2];
         if constexpr (FMT == BF_NVFP4) {
-          const uint32_t word = p < 2 ? now.x : now.y;
           uint32_t h;
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(word >> (16 * (p & 1)))));
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(now >> (16 * p))));
           m[0] = __byte_perm(h, 0, 0x1010);
           m[1] = __byte_perm(h, 0, 0x3232);
         } else {
-          const uint32_t s = (now.x >> (8 * (FMT == BF_MXF8 ? p / 2 : p))) & 0xFFu;
-          const int d = (int)s - (int)ref;
-          m[0] = s == 255u ? 0x7E007E00u : (uint32_t)(d + 15) * 0x04000400u;
-          if (d < -14) {
+          // a block is two 16-byte pieces of 8-bit codes, one of 4-bit codes
+          const uint32_t s = (now >> (8 * (FMT == BF_MXF8 ? p / 2 : p))) & 0xFFu;
+          m[0] = s == 255u ? 0x7E007E00u : (uint32_t)((int)s - (int)ref + 15) * 0x04000400u;
+          if (far_scale<FMT>(s, ref)) {
             m[0] = 0u;
-            if ((c[0] | c[1] | c[2] | c[3]) & (FMT == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) {
-              if (!any_far) {
-                any_far = true;
-                has_far[half][r] = 1;
-                for (int t = 0; t < sh.tokens; ++t) far[t] = 0.0f;
-              }
-              far_block<FMT>(c, s, slot + kRows * kCodeBytes, sh.tokens, piece * elems, far);
-            }
+            any_far |= any_code(FMT, make_uint4(c[0], c[1], c[2], c[3]));
           }
           m[1] = m[0];
         }
@@ -382,7 +407,6 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           }
         }
         const uint32_t to = tmem_a + b * a_cols + lanes + piece * (elems / 2);
-        __syncwarp();  // lanes with far blocks took longer
         if constexpr (FMT == BF_MXF8) {
           asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(to),
                        "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]), "r"(f[4]), "r"(f[5]), "r"(f[6]), "r"(f[7])
@@ -400,6 +424,13 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         round ^= 1u;
       }
     }
+    if constexpr (FMT != BF_NVFP4) {
+      has_far[pt][r] = any_far;
+      // x has been read through the ring, so the kernel that laid it out has ended
+      if (any_far && !aborted)
+        far_blocks<FMT>(a, x16 + (int64_t)token0 * sh.steps * sk, (int64_t)sh.steps * sk, row, s0, s1, pt,
+                        ref, cols, far);
+    }
   }
 
   tc_fence_before();
@@ -409,12 +440,11 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const int64_t at = (int64_t)blockIdx.y * sh.row_tiles + tile;
   float* mine = part + (at * sh.slices + slice) * ((int64_t)sh.tokens * kRows);
   if (warp < kDecodeWarps && !aborted) {
-    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int pt = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const float scale = FMT == BF_NVFP4 ? 1.0f : ref_scale[r];
-    const bool far0 = FMT != BF_NVFP4 && has_far[0][r], far1 = FMT != BF_NVFP4 && has_far[1][r];
-    const float* f0 = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2) * kRows + r) * 128;
-    for (int c = half * 16; c < sh.tokens; c += 32) {
+    const float* f0 = far_ws + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kParts * kRows + r) * 128;
+    for (int c = pt * 16; c < sh.tokens; c += 16 * kParts) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + lanes + c, v);
       tmem_ld_wait();
@@ -424,8 +454,11 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (t >= cols) break;
         const float d = __uint_as_float(v[i]);
         float sum = FMT == BF_NVFP4 || d == 0.0f ? d : d * scale;
-        if (far0) sum += __ldcg(f0 + t);
-        if (far1) sum += __ldcg(f0 + kRows * 128 + t);
+        if constexpr (FMT != BF_NVFP4) {
+#pragma unroll
+          for (int q = 0; q < kParts; ++q)
+            if (has_far[q][r]) sum += __ldcg(f0 + q * (kRows * 128) + t);
+        }
         if (sh.slices > 1)
           __stcg(mine + t * kRows + r, sum);
         else if (row0 + r < n)
@@ -449,14 +482,26 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   if (!last) return;
   __threadfence();
   const float* all = part + at * sh.slices * ((int64_t)sh.tokens * kRows);
-  for (int e = threadIdx.x; e < cols * kRows; e += kThreads) {
-    const int t = e / kRows, r = e % kRows;
-    float sum = 0.0f;
+  // four rows of a token at a time
+  const int64_t stride = (int64_t)sh.tokens * kRows / 4;
+#pragma unroll 2
+  for (int e = threadIdx.x; e < cols * (kRows / 4); e += kThreads) {
+    const int t = e / (kRows / 4), r = e % (kRows / 4) * 4;
+    const float4* p = reinterpret_cast<const float4*>(all) + e;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int k = 0; k < sh.slices; ++k) sum += __ldcg(all + (int64_t)k * sh.tokens * kRows + e);
-    if (row0 + r < n)
-      static_cast<T*>(a.out)[(int64_t)(token0 + t) * a.ld_out + row0 + r] =
-          from_f32<T>(a.alpha * (sum * __ldcg(xs + token0 + t)));
+    for (int k = 0; k < sh.slices; ++k) {
+      const float4 q = __ldcg(p + k * stride);
+      sum.x += q.x;
+      sum.y += q.y;
+      sum.z += q.z;
+      sum.w += q.w;
+    }
+    const float s = __ldcg(xs + token0 + t), v[4] = {sum.x, sum.y, sum.z, sum.w};
+    T* dst = static_cast<T*>(a.out) + (int64_t)(token0 + t) * a.ld_out + row0 + r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (row0 + r + i < n) dst[i] = from_f32<T>(a.alpha * (v[i] * s));
   }
 }
 
@@ -467,13 +512,13 @@ TileShape tile_shape(int fmt, const FewLinearArgs& a, int sm_count) {
   s.z = (int)((a.T + 127) / 128);
   s.steps = (int)((a.kp + step_k(fmt) - 1) / step_k(fmt));
   s.row_tiles = (int)((a.N + kRows - 1) / kRows);
-  const int scales = step_k(fmt) / 2 / bf_block(fmt);  // a thread's of a step
+  const int scales = step_k(fmt) / bf_block(fmt);  // of a row in a step
   s.words = a.kp / bf_block(fmt) % scales == 0 && (reinterpret_cast<uintptr_t>(a.sf) % scales) == 0;
   // one CTA an SM; K is cut as far as there are SMs left and each CTA keeps two steps
   int n = sm_count / (s.row_tiles * s.z);
   n = n < s.steps / 2 ? n : s.steps / 2;
   s.slices = n < 1 ? 1 : n;
-  const int slot = kRows * kCodeBytes + s.tokens * step_k(fmt) * 2;
+  const int slot = kRows * kCodeBytes + s.tokens * step_k(fmt) * 2 + kScaleBytes;
   s.stages = (220 * 1024) / slot < kMaxStages ? (220 * 1024) / slot : kMaxStages;
   s.smem = s.stages * slot + 1024;
   // tensor memory is taken whole: one CTA an SM
@@ -493,7 +538,7 @@ TileWs tile_ws(int fmt, const FewLinearArgs& a, const TileShape& s) {
   w.xs = up256((size_t)a.T * s.steps * step_k(fmt) * 2);
   w.far = w.xs + up256((size_t)a.T * sizeof(float));
   const size_t ctas = (size_t)s.row_tiles * s.slices * s.z;
-  w.part = w.far + (fmt == BF_NVFP4 ? 0 : ctas * 2 * kRows * 128 * sizeof(float));
+  w.part = w.far + (fmt == BF_NVFP4 ? 0 : ctas * kParts * kRows * 128 * sizeof(float));
   w.total = w.part + (s.slices > 1 ? ctas * s.tokens * kRows * sizeof(float) : 0);
   return w;
 }
@@ -520,7 +565,8 @@ cudaError_t tiles_launch(const FewLinearArgs& a, const TileShape& sh, const CUte
   cfg.stream = s;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, few_tiles_kernel<T, FMT>, mw, mx, a, sh, static_cast<const float*>(xs),
+  return cudaLaunchKernelEx(&cfg, few_tiles_kernel<T, FMT>, mw, mx, a, sh,
+                            reinterpret_cast<const __half*>(ws + w.x16), static_cast<const float*>(xs),
                             reinterpret_cast<float*>(ws + w.part), reinterpret_cast<float*>(ws + w.far));
 }
 
