@@ -105,35 +105,18 @@ class Engine(LinearOps):
               stages=0, max_ctas=0, ab_mode=0, sparse=0, meta=None, sfa=None, sfb=None,
               lda=None, ldb=None, ldc=None, meta_layout=0, raster_m=0, m_sub=0,
               split_tail=0, b_format=0, mx_scale=0, instruction=0):
-        d = GemmDesc()
-        d.format = fmt
-        d.sparse = sparse
         # stored elements per 8 bits of a row (1 for the byte and wider formats,
         # whose tensors hold whole elements)
-        sub = {FMT_E2M1: 4, FMT_MXF4: 4, FMT_NVFP4: 4, FMT_E2M3: 6, FMT_E3M2: 6}
-        bits, b_bits = sub.get(fmt, 8), sub.get(b_format or fmt, 8)
-        elems = lambda nbytes: nbytes * 8 // bits
-        d.M = M if M is not None else A.shape[0]
-        d.N = N if N is not None else B.shape[0]
+        bits, b_bits = _PACKED_BITS.get(fmt, 8), _PACKED_BITS.get(b_format or fmt, 8)
         if K is None:
-            K = elems(A.shape[1]) * (2 if sparse else 1)
-        d.K = K
-        d.lda = lda if lda is not None else elems(A.stride(0))
-        d.ldb = ldb if ldb is not None else B.stride(0) * 8 // b_bits
-        d.b_format = b_format
-        d.mx_scale = mx_scale
-        d.instruction = instruction
-        d.ldc = ldc if ldc is not None else C_out.stride(0)
-        d.A, d.B, d.C = _ptr(A), _ptr(B), _ptr(C_out)
-        d.sfa, d.sfb, d.meta = _ptr(sfa), _ptr(sfb), _ptr(meta)
-        d.alpha = alpha
-        d.cta_group, d.ab_mode, d.tile_n, d.stages, d.max_ctas = (
-            cta_group, ab_mode, tile_n, stages, max_ctas)
-        d.meta_layout = meta_layout
-        d.raster_m = raster_m
-        d.m_sub = m_sub
-        d.split_tail = split_tail
-        return d
+            K = A.shape[1] * 8 // bits * (2 if sparse else 1)
+        return GemmDesc(
+            fmt, sparse, M if M is not None else A.shape[0], N if N is not None else B.shape[0], K,
+            lda if lda is not None else A.stride(0) * 8 // bits,
+            ldb if ldb is not None else B.stride(0) * 8 // b_bits,
+            ldc if ldc is not None else C_out.stride(0), _ptr(A), _ptr(B), _ptr(C_out), _ptr(sfa),
+            _ptr(sfb), _ptr(meta), alpha, cta_group, ab_mode, tile_n, stages, max_ctas, meta_layout,
+            raster_m, m_sub, split_tail, b_format, mx_scale, instruction)
 
     def gemm_host(self, A, B, C_out, fmt: int, *, alpha: float = 1.0, stream=None, **kw):
         """b2g_gemm_host: A, B, C_out are HOST tensors (pin them for full copy speed);

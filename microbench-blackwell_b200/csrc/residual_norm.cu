@@ -45,9 +45,10 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
     const T* lo = static_cast<const T*>(p);
     return load8_any<T, ANY>(row + col[j], n[j], lo, lo + ((rows - 1) * ld + cols));
   };
-  auto put = [&](void* p, int64_t ld, int j, const float(&f)[8]) {
+  auto put = [&](void* p, int64_t ld, int j, const float2(&f)[4]) {
     const int left = cols - (col[j] - (int)(threadIdx.x & 31) * 8);
-    store8_any<T, ANY>(static_cast<T*>(p) + row * ld + col[j], f, n[j],
+    const float o[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
+    store8_any<T, ANY>(static_cast<T*>(p) + row * ld + col[j], o, n[j],
                        left < 0 ? 0 : left < 256 ? left : 256, buf);
   };
 #pragma unroll
@@ -55,18 +56,19 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
     rx[j] = get(a.x, x, a.rows, a.ld_x, j);
     if (a.y) ry[j] = get(a.y, y, a.rows, a.ld_y, j);
   }
-  float v[NV][8];
+  float2 v[NV][4];
   if (a.y) {
     float r1 = 1.0f;
     if (a.w_post) {
-      float ss[1] = {0.0f};
+      float2 sum = both(0.0f);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        float f[8];
-        unpack8(ry[j], f);
+        float2 f[4];
+        unpack4x2(ry[j], f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss[0] = fmaf(f[i], f[i], ss[0]);
+        for (int i = 0; i < 4; ++i) sum = fma2(f[i], f[i], sum);
       }
+      float ss[1] = {sum.x + sum.y};
       row_sum(ss, red[0]);
       r1 = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
       if (a.rstd_post && threadIdx.x == 0) a.rstd_post[row] = r1;
@@ -74,66 +76,64 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
     const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float fx[8], fy[8];
-      unpack8(rx[j], fx);
-      unpack8(ry[j], fy);
+      float2 fx[4], fy[4];
+      unpack4x2(rx[j], fx);
+      unpack4x2(ry[j], fy);
       if (a.w_post) {
-        float w[8];
-        unpack8(get(a.w_post, static_cast<const T*>(a.w_post), 1, 0, j), w);
+        float2 w[4];
+        unpack4x2(get(a.w_post, static_cast<const T*>(a.w_post), 1, 0, j), w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) fy[i] = fy[i] * r1 * w[i];
+        for (int i = 0; i < 4; ++i) fy[i] = mul2(mul2(fy[i], both(r1)), w[i]);
       }
       if (gate) {
-        float g[8];
-        unpack8(get(a.gate, gate, (a.rows - 1) / a.rows_per_gate + 1, a.cols, j), g);
+        float2 g[4];
+        unpack4x2(get(a.gate, gate, (a.rows - 1) / a.rows_per_gate + 1, a.cols, j), g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) fy[i] *= g[i];
+        for (int i = 0; i < 4; ++i) fy[i] = mul2(fy[i], g[i]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = fmaf(a.beta, fy[i], a.alpha * fx[i]);
+      for (int i = 0; i < 4; ++i) v[j][i] = fma2(both(a.beta), fy[i], mul2(both(a.alpha), fx[i]));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      unpack8(rx[j], v[j]);
+      unpack4x2(rx[j], v[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] *= a.alpha;
+      for (int i = 0; i < 4; ++i) v[j][i] = mul2(v[j][i], both(a.alpha));
     }
   }
   if (a.x_out) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      put(a.x_out, a.ld_x_out, j, v[j]);
+    for (int j = 0; j < NV; ++j) put(a.x_out, a.ld_x_out, j, v[j]);
   }
   if (!a.w_pre) return;
-  float ss[1] = {0.0f};
+  float2 sum = both(0.0f);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss[0] = fmaf(v[j][i], v[j][i], ss[0]);
+    for (int i = 0; i < 4; ++i) sum = fma2(v[j][i], v[j][i], sum);
+  float ss[1] = {sum.x + sum.y};
   row_sum(ss, red[1]);
   const float r2 = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
   if (a.rstd_pre && threadIdx.x == 0) a.rstd_pre[row] = r2;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    float w[8];
-    unpack8(get(a.w_pre, static_cast<const T*>(a.w_pre), 1, 0, j), w);
+    float2 w[4];
+    unpack4x2(get(a.w_pre, static_cast<const T*>(a.w_pre), 1, 0, j), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * r2 * w[i];
+    for (int i = 0; i < 4; ++i) v[j][i] = mul2(mul2(v[j][i], both(r2)), w[i]);
     if (a.h) put(a.h, a.ld_h, j, v[j]);
     if constexpr (HF >= 0) {
       constexpr int blk = bf_block(HF), bits = bf_bits(HF);
       constexpr int mode = HF == BF_NVFP4 ? Q_DIVIDE : Q_EXACT;
       float amax = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[j][i]));
+      for (int i = 0; i < 4; ++i) amax = max_nan(amax, max_nan(fabsf(v[j][i].x), fabsf(v[j][i].y)));
       amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
       if constexpr (blk == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
       const BlockScale s = block_scale<HF, mode>(amax);
-      const float2 x2[4] = {make_float2(v[j][0], v[j][1]), make_float2(v[j][2], v[j][3]),
-                            make_float2(v[j][4], v[j][5]), make_float2(v[j][6], v[j][7])};
       uint32_t q[2];
-      encode8<HF, mode, false>(x2, s, 1.0f, make_uint2(0, 0), q);
+      encode8<HF, mode, false>(v[j], s, 1.0f, make_uint2(0, 0), q);
       if (col[j] < a.kp) {
         const int64_t e = row * a.kp + col[j];
         if constexpr (HF == BF_MXF8)
