@@ -225,26 +225,22 @@ __device__ __forceinline__ uint4 shift16(const uint4& x, const uint4& y, uint32_
 }
 
 // load8 for rows of any alignment (ANY; else every p is 16-byte aligned): aligned words
-// shifted together where they lie within the operand [lo, hi), else element by element.
+// shifted together where they lie within the operand, else element by element.  `inside`:
+// the row has others of 16 elements or more before and behind it, so they do.
 template <typename T, bool ANY>
-__device__ __forceinline__ Raw8<T> load8_any(const T* p, int n, const T* lo, const T* hi) {
+__device__ __forceinline__ Raw8<T> load8_any(const T* p, int n, bool inside) {
   if constexpr (ANY) {
     const uint32_t m = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
     if (m && n >= 8) {
-      Raw8<T> r;
-      if constexpr (sizeof(T) == 4) {
-        uint32_t u[8];
-        if (load32_any(p, lo, hi, u)) {
-          r.w[0] = make_uint4(u[0], u[1], u[2], u[3]);
-          r.w[1] = make_uint4(u[4], u[5], u[6], u[7]);
-          return r;
-        }
-      } else {
+      if (inside) {
+        Raw8<T> r;
         const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - m);
-        if (q >= static_cast<const void*>(lo) && q + 2 <= static_cast<const void*>(hi)) {
-          r.w[0] = shift16(__ldg(q), __ldg(q + 1), m);
-          return r;
-        }
+        uint4 w[sizeof(T) / 2 + 1];
+#pragma unroll
+        for (int i = 0; i <= (int)sizeof(T) / 2; ++i) w[i] = __ldg(q + i);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = shift16(w[i], w[i + 1], m);
+        return r;
       }
       return load8(p, n, false);
     }

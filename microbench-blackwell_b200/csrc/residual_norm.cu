@@ -40,10 +40,9 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
     const int left = cols - col[j];
     n[j] = left < 0 ? 0 : left < 8 ? left : 8;
   }
-  // eight elements of a row of an operand that has `rows` rows, ld apart
-  auto get = [&](const void* p, const T* row, int64_t rows, int64_t ld, int j) {
-    const T* lo = static_cast<const T*>(p);
-    return load8_any<T, ANY>(row + col[j], n[j], lo, lo + ((rows - 1) * ld + cols));
+  // eight elements of row r of an operand that has `rows` rows
+  auto get = [&](const T* at, int64_t r, int64_t rows, int j) {
+    return load8_any<T, ANY>(at + col[j], n[j], cols >= 16 && r > 0 && r < rows - 1);
   };
   auto put = [&](void* p, int64_t ld, int j, const float2(&f)[4]) {
     const int left = cols - (col[j] - (int)(threadIdx.x & 31) * 8);
@@ -53,8 +52,8 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
   };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    rx[j] = get(a.x, x, a.rows, a.ld_x, j);
-    if (a.y) ry[j] = get(a.y, y, a.rows, a.ld_y, j);
+    rx[j] = get(x, row, a.rows, j);
+    if (a.y) ry[j] = get(y, row, a.rows, j);
   }
   float2 v[NV][4];
   if (a.y) {
@@ -73,7 +72,8 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
       r1 = 1.0f / sqrtf(ss[0] / (float)a.cols + a.eps);
       if (a.rstd_post && threadIdx.x == 0) a.rstd_post[row] = r1;
     }
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
+    const int64_t gate_row = row / a.rows_per_gate, last_gate = (a.rows - 1) / a.rows_per_gate;
+    const T* gate = a.gate ? static_cast<const T*>(a.gate) + gate_row * a.cols : nullptr;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float2 fx[4], fy[4];
@@ -81,13 +81,13 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
       unpack4x2(ry[j], fy);
       if (a.w_post) {
         float2 w[4];
-        unpack4x2(get(a.w_post, static_cast<const T*>(a.w_post), 1, 0, j), w);
+        unpack4x2(get(static_cast<const T*>(a.w_post), 0, 1, j), w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) fy[i] = mul2(mul2(fy[i], both(r1)), w[i]);
       }
       if (gate) {
         float2 g[4];
-        unpack4x2(get(a.gate, gate, (a.rows - 1) / a.rows_per_gate + 1, a.cols, j), g);
+        unpack4x2(get(gate, gate_row, last_gate + 1, j), g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) fy[i] = mul2(fy[i], g[i]);
       }
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     float2 w[4];
-    unpack4x2(get(a.w_pre, static_cast<const T*>(a.w_pre), 1, 0, j), w);
+    unpack4x2(get(static_cast<const T*>(a.w_pre), 0, 1, j), w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[j][i] = mul2(mul2(v[j][i], both(r2)), w[i]);
     if (a.h) put(a.h, a.ld_h, j, v[j]);

@@ -96,9 +96,9 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
       store4x2(row + col[j], f, true);
     }
   };
-  auto get = [&](const void* p, int64_t at, int64_t elements, int j) {
-    const T* lo = static_cast<const T*>(p);
-    return load8_any<T, ANY>(lo + at + col[j], ANY ? n[j] : on[j] ? 8 : 0, lo, lo + elements);
+  auto get = [&](const void* p, int64_t r, int64_t rows, int j) {  // of row r, cols apart
+    return load8_any<T, ANY>(static_cast<const T*>(p) + r * cols + col[j], ANY ? n[j] : on[j] ? 8 : 0,
+                             cols >= 16 && r > 0 && r < rows - 1);
   };
   // row r of a tensor with leading dimension ld: the same for the CTA, columns are added
   auto row_of = [](auto* p, int64_t ld, int64_t r) { return p + r * ld; };
@@ -109,10 +109,12 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
       const int words = (int)((at - first) + cols * sizeof(T) + 15) / 16;
       const uintptr_t lo = reinterpret_cast<uintptr_t>(p),
                       hi = reinterpret_cast<uintptr_t>(p + ((rows - 1) * ld + cols));
+      // with rows before and behind, all words are the operand's
+      const bool inside = cols >= 16 && r > 0 && r < rows - 1;
       for (int k = tid; k < words; k += nt) {
         const uintptr_t q = first + 16 * (uintptr_t)k;
         const uint32_t to = slot + tensor * kTensor + 16 * k;
-        if (q >= lo && q + 16 <= hi) {
+        if (inside || (q >= lo && q + 16 <= hi)) {
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(q) : "memory");
         } else {  // an end of the operand: its elements alone
           for (int i = 0; i < 16; i += (int)sizeof(T))
@@ -184,7 +186,7 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
   Raw8<T> wq[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
-    if (kKeep && has_h) wq[j] = get(a.w_pre, 0, cols, j);
+    if (kKeep && has_h) wq[j] = get(a.w_pre, 0, 1, j);
   float2 dwq[NV][4], dwp[NV][4], z[NV][4], gw[NV][4];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -203,11 +205,11 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
   };
   auto post_of = [&](int j, float2 (&f)[4]) {
     ones(f);
-    if (norm_y) unpack4x2(get(a.w_post, 0, cols, j), f);
+    if (norm_y) unpack4x2(get(a.w_post, 0, 1, j), f);
   };
   auto gate_of = [&](int64_t g, int j, float2 (&f)[4]) {
     ones(f);
-    if (a.gate) unpack4x2(get(a.gate, g * a.cols, gates * a.cols, j), f);
+    if (a.gate) unpack4x2(get(a.gate, g, gates, j), f);
   };
   // gradients of the gate that ends before row r (its last row here is r - 1)
   auto leave_gate = [&](int64_t r) {
@@ -315,7 +317,7 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
         float2 p[4], w[4];
         fetch(slot, 0, j, p);
         fetch(slot, 1, j, v);
-        unpack4x2(kKeep ? wq[j] : get(a.w_pre, 0, cols, j), w);
+        unpack4x2(kKeep ? wq[j] : get(a.w_pre, 0, 1, j), w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           dwq[j][i] = fma2(p[i], mul2(v[i], both(r2)), dwq[j][i]);
@@ -527,8 +529,8 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradAr
     const int n = cols - c < 8 ? cols - c : 8;
     // columns c .. of row r of an operand with `rows` rows, ld apart
     auto get = [&](const void* p, int64_t r, int64_t ld, int64_t rows, float (&f)[8]) {
-      const T* lo = static_cast<const T*>(p);
-      unpack8(load8_any<T, ANY>(lo + r * ld + c, n, lo, lo + ((rows - 1) * ld + cols)), f);
+      unpack8(load8_any<T, ANY>(static_cast<const T*>(p) + r * ld + c, n,
+                                cols >= 16 && r > 0 && r < rows - 1), f);
     };
     float p[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (a.dh) {
@@ -618,8 +620,8 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
   const int count = cols - c0 < 256 ? cols - c0 : 256;
   // columns c .. of row r of an operand with `rows` rows, ld apart
   auto get = [&](const void* p, int64_t r, int64_t ld, int64_t rows, float (&f)[8]) {
-    const T* lo = static_cast<const T*>(p);
-    unpack8(load8_any<T, ANY>(lo + r * ld + c, n, lo, lo + ((rows - 1) * ld + cols)), f);
+    unpack8(load8_any<T, ANY>(static_cast<const T*>(p) + r * ld + c, n,
+                              cols >= 16 && r > 0 && r < rows - 1), f);
   };
   auto put = [&](void* p, int64_t r, int64_t ld, const float(&f)[8]) {
     store8_any<T, ANY>(static_cast<T*>(p) + r * ld + c, f, n, count, stores[ANY ? ry : 0]);
