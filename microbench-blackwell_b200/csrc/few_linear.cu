@@ -1,9 +1,9 @@
-// few_linear.cu -- y = alpha * x . W^T of a few tokens (16-bit x) with microscaled
+// few_linear.cu -- y = alpha * x . W^T of one to eight tokens (16-bit x) with microscaled
 // weights, for decoding: every weight is read once and used a handful of times, so the
 // kernel is bound by the weights' bytes.
 //
 // Codes become fp16 pairs in registers and go into mma.sync m16n8k16 with the weights
-// as the 16-row operand and up to 8 tokens as the 8 columns: tcgen05 takes its operands
+// as the 16-row operand and the tokens as the 8 columns: tcgen05 takes its operands
 // from shared or tensor memory, so a decoded weight would have to be stored first, for
 // products whose own time does not count at this many tokens.  e2m1 and e4m3 values and
 // e2m1 * ue4m3 products are exact in fp16; sums are fp32.  A first kernel lays x out as
@@ -173,11 +173,11 @@ struct Ring {
 
 // c += codes of one group, times the fp16 pairs m, times x.  m[i]: multipliers of row
 // g + 8 i for the first and the second half of the thread's elements.  xf: shared address
-// of the lane's fragments, one step pair and token tile `step` bytes after the other, their
-// 16-byte place xor'ed with the step pair where swz is set.
-template <int FMT, int NT>
+// of the lane's fragments, one step pair `step` bytes after the other, their 16-byte place
+// xor'ed with the step pair where swz is set.
+template <int FMT>
 __device__ __forceinline__ void codes_mma(const GroupData<FMT>& d, const uint32_t (&m)[2][2],
-                                          uint32_t xf, uint32_t step, uint32_t swz, float (&c)[NT][4]) {
+                                          uint32_t xf, uint32_t step, uint32_t swz, float (&c)[4]) {
 #pragma unroll
   for (int jp = 0; jp < kPairs; ++jp) {
     uint32_t f[2][4];
@@ -189,29 +189,24 @@ __device__ __forceinline__ void codes_mma(const GroupData<FMT>& d, const uint32_
       for (int k = 0; k < 4; ++k)
         f[k >> 1][i + 2 * (k & 1)] = mul_h2(p[k], m[i][jp < kPairs / 2 ? 0 : 1]);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint4 b = shared_at<uint4>((xf ^ (swz & (16u * jp))) + (n * kPairs + jp) * step);
-      mma_f16(c[n], f[0], b.x, b.y);
-      mma_f16(c[n], f[1], b.z, b.w);
-    }
+    const uint4 b = shared_at<uint4>((xf ^ (swz & (16u * jp))) + jp * step);
+    mma_f16(c, f[0], b.x, b.y);
+    mma_f16(c, f[1], b.z, b.w);
   }
 }
 
 // Sums of a warp.  NVFP4: scales are multiplied into the codes, sums are final.  MX: an
 // E8M0 scale has more range than fp16, so codes are multiplied by 2^(s - ref) with one
 // ref for each row, and the sum by 2^ref in fp32 when ref changes and at the end.
-template <int FMT, int NT>
+template <int FMT>
 struct Sums {
-  float c[NT][4];
-  float total[NT][4];  // MX: what earlier refs summed up
-  int ref[2];          // MX: of rows g and g + 8, the same in a quad
+  float c[4];
+  float total[4];  // MX: what earlier refs summed up
+  int ref[2];      // MX: of rows g and g + 8, the same in a quad
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[n][i] = total[n][i] = 0.0f;
+    for (int i = 0; i < 4; ++i) c[i] = total[i] = 0.0f;
     ref[0] = ref[1] = 127;
   }
 
@@ -219,13 +214,10 @@ struct Sums {
   __device__ __forceinline__ void flush() {
     const float s0 = e8m0_value((uint32_t)ref[0]), s1 = e8m0_value((uint32_t)ref[1]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // a sum that is still zero stays zero, whatever its ref
-        if (c[n][i] != 0.0f) total[n][i] = fmaf(i < 2 ? s0 : s1, c[n][i], total[n][i]);
-        c[n][i] = 0.0f;
-      }
+    for (int i = 0; i < 4; ++i) {
+      // a sum that is still zero stays zero, whatever its ref
+      if (c[i] != 0.0f) total[i] = fmaf(i < 2 ? s0 : s1, c[i], total[i]);
+      c[i] = 0.0f;
     }
   }
 
@@ -254,7 +246,7 @@ struct Sums {
         m[i][0] = m[i][1] = (uint32_t)((int)d.s[i] - ref[i] + 15) * 0x04000400u;
       }
     }
-    codes_mma<FMT, NT>(d, m, xf, step, swz, c);
+    codes_mma<FMT>(d, m, xf, step, swz, c);
   }
 
   // Any group: the largest scale of each row's four threads becomes ref.  Blocks of zeros
@@ -287,7 +279,7 @@ struct Sums {
         const uint32_t e = (uint32_t)(max(s[i] - top[i], -14) + 15) * 0x04000400u;
         m[i][0] = m[i][1] = !wide ? e : t != p ? 0u : s[i] == 255 ? 0x7E007E00u : 0x3C003C00u;
       }
-      codes_mma<FMT, NT>(d, m, xf, step, swz, c);
+      codes_mma<FMT>(d, m, xf, step, swz, c);
     }
   }
 };
@@ -295,12 +287,11 @@ struct Sums {
 // Work of a launch.  K is cut into `slices`; CTA c keeps slice c % slices and has that part
 // of x in shared memory.  k_split 1: each warp takes row blocks of 16 by itself, every
 // (rows_ctas * kWarps)-th one.  k_split kWarps: the warps of a CTA share a row block and
-// cut its K among them.  blockIdx.y: groups of 8 * NT tokens.
+// cut its K among them.
 struct FewShape {
-  int steps, slices, rows_ctas, z, k_split;
+  int steps, slices, rows_ctas, k_split;
   int groups;      // of 128 elements, whole steps
   int words;       // rows of scales start on 4 bytes
-  int tile_cols;   // columns of a token tile laid out: 8, or the tokens there are
   int x_bytes;     // shared memory of a CTA's part of x
 };
 
@@ -308,16 +299,15 @@ struct FewShape {
 // covers the memory's latency at its rate.
 constexpr int kAhead = 4;
 
-// x as fp16 B fragments: [token group][group][token tile][step pair][4 threads][column] of
-// 16 bytes, the four elements of two steps; xs[token] = the power of two to undo.  In a
-// full tile column c of thread t and pair jp lies at c ^ (jp + 4 (t % 2)): the lanes that
+// x as fp16 B fragments: [group][step pair][4 threads][token] of 16 bytes, the four
+// elements of two steps; xs[token] = the power of two to undo.  Of eight tokens column c of thread t and pair jp lies at c ^ (jp + 4 (t % 2)): the lanes that
 // read it, and the eight neighbours that write one column, meet different banks.  Zero past
 // K up to the end of the last group.  One CTA per token.
-template <typename T, int NT>
+template <typename T>
 __global__ void __launch_bounds__(512) few_prepare_kernel(const FewLinearArgs a, const FewShape sh,
                                                           uint4* frag, float* xs) {
   __shared__ float red[16];
-  const int token = blockIdx.x, z = token / (8 * NT), tile = token / 8 % NT, col = token & 7;
+  const int token = blockIdx.x, tokens = (int)a.T;
   const int vecs = sh.groups * (kGroup / 8);
   const T* x = static_cast<const T*>(a.x) + (int64_t)token * a.ld_x;
   // the product kernel may start and load weights; it waits for this one to end before
@@ -365,7 +355,6 @@ __global__ void __launch_bounds__(512) few_prepare_kernel(const FewLinearArgs a,
   auto put = [&](int v, const Raw8<T>& r) {
     // eight elements: one step pair of one thread
     const int in = v % (kGroup / 8), jp = in % kPairs, t = in / kPairs;
-    const int64_t group = (int64_t)z * sh.groups + v / (kGroup / 8);
     uint4 w = r.w[0];
     if constexpr (__is_same(T, __nv_bfloat16)) {
       float f[8];
@@ -375,8 +364,8 @@ __global__ void __launch_bounds__(512) few_prepare_kernel(const FewLinearArgs a,
       w.z = pack2<__half>(f[4] * scale, f[5] * scale);
       w.w = pack2<__half>(f[6] * scale, f[7] * scale);
     }
-    const int place = sh.tile_cols == 8 ? col ^ (jp | (t & 1) << 2) : col;
-    frag[(((group * NT + tile) * kPairs + jp) * 4 + t) * sh.tile_cols + place] = w;
+    const int place = tokens == 8 ? token ^ (jp | (t & 1) << 2) : token;
+    frag[((v / (kGroup / 8) * kPairs + jp) * 4 + t) * tokens + place] = w;
   };
 #pragma unroll
   for (int i = 0; i < kHold; ++i) {
@@ -386,15 +375,15 @@ __global__ void __launch_bounds__(512) few_prepare_kernel(const FewLinearArgs a,
   for (int i = kHold, v = threadIdx.x + kHold * 512; v < vecs; ++i, v += 512) put(v, at(v, i));
 }
 
-template <typename T, int FMT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT <= 4 ? 2 : 1)
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kWarps * 32, 2)
 few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, const float* xs,
                   float* part) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[2][kWarps][NT == 1 ? 128 : 1];  // k_split: sums of the warps
+  __shared__ float red[2][kWarps][128];  // k_split: sums of the warps
   constexpr int kSlots = kAhead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool split = NT == 1 && sh.k_split > 1;
+  const bool split = sh.k_split > 1;
   const int slice = (int)blockIdx.x % sh.slices;
   // steps of this CTA and of this warp
   const int cb = (int)((unsigned)sh.steps * (unsigned)slice / (unsigned)sh.slices);
@@ -428,17 +417,15 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
 #pragma unroll 1
   for (int u = 0; u < kSlots; ++u) ask(u);
 
-  const int64_t token0 = (int64_t)blockIdx.y * (8 * NT);
-  const int cols = a.T - token0 < 8 * NT ? (int)(a.T - token0) : 8 * NT;
-  const uint32_t step = 64 * sh.tile_cols;  // bytes of an MMA step pair of a token tile
-  const uint32_t group_bytes = NT * kPairs * step;
+  const int cols = (int)a.T;
+  const uint32_t step = 64 * cols;  // bytes of an MMA step pair
+  const uint32_t group_bytes = kPairs * step;
   constexpr int kParts = few_groups(FMT);
   const uint32_t x_smem = (uint32_t)__cvta_generic_to_shared(smem);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {
     const uint32_t bytes = (uint32_t)(ce - cb) * kParts * group_bytes;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(frag) +
-                         ((int64_t)blockIdx.y * sh.steps + cb) * kParts * group_bytes;
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(frag) + (int64_t)cb * kParts * group_bytes;
     for (uint32_t i = threadIdx.x * 16; i < bytes; i += kWarps * 32 * 16)
       cp_async16(x_smem + i, src + i, true);
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -447,14 +434,13 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
   }
 
   // columns past T repeat another one's or hold anything, and are not stored
-  const uint32_t swz = sh.tile_cols == 8 ? 0x70u : 0u;
+  const uint32_t swz = cols == 8 ? 0x70u : 0u;
   const uint32_t xf0 = x_smem + (uint32_t)(gb - cb) * kParts * group_bytes +
-                       (t * sh.tile_cols + (sh.tile_cols == 8 ? g ^ (t & 1) << 2
-                                            : g < sh.tile_cols ? g : 0)) * 16;
+                       (t * cols + (cols == 8 ? g ^ (t & 1) << 2 : g < cols ? g : 0)) * 16;
   int slot = 0, turn = 0;
 #pragma unroll 1
   for (int rb = rb0; rb < row_blocks; rb += rb_step, turn ^= 1) {
-    Sums<FMT, NT> sums;
+    Sums<FMT> sums;
     sums.clear();
     uint32_t xf = xf0;
 #pragma unroll 1
@@ -479,25 +465,24 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
     if constexpr (FMT != BF_NVFP4) sums.flush();
 
     // accumulator i of lane (g, t): row g + 8 (i / 2), token 2 t + i % 2
-    const float(&sum)[NT][4] = FMT == BF_NVFP4 ? sums.c : sums.total;
-    const int64_t at = (int64_t)blockIdx.y * row_blocks + rb;
-    float* mine = part + (at * sh.slices + slice) * (NT * 128);
+    const float(&sum)[4] = FMT == BF_NVFP4 ? sums.c : sums.total;
+    float* mine = part + ((int64_t)rb * sh.slices + slice) * 128;
     auto put = [&](int token, int row, float s) {
       if (token < cols && row < (int)a.N)
-        static_cast<T*>(a.out)[(token0 + token) * a.ld_out + row] = from_f32<T>(a.alpha * s);
+        static_cast<T*>(a.out)[token * a.ld_out + row] = from_f32<T>(a.alpha * s);
     };
     if (split) {
       // two buffers: a warp writes one again only after the barrier of the other
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        red[turn][warp][(2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = sum[0][i];
+        red[turn][warp][(2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = sum[i];
       __syncthreads();
       const int e = threadIdx.x;
       if (e < cols * 16) {
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) s += red[turn][w][e];
-        s *= xs[token0 + e / 16];
+        s *= xs[e / 16];
         if (sh.slices == 1)
           put(e / 16, rb * 16 + e % 16, s);
         else
@@ -505,21 +490,19 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
       }
     } else {
 #pragma unroll
-      for (int n8 = 0; n8 < NT; ++n8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int token = n8 * 8 + 2 * t + (i & 1), r = g + 8 * (i >> 1);
-          if (token >= cols) continue;
-          const float s = sum[n8][i] * xs[token0 + token];
-          if (sh.slices == 1)
-            put(token, rb * 16 + r, s);
-          else
-            __stcg(mine + token * 16 + r, s);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int token = 2 * t + (i & 1), r = g + 8 * (i >> 1);
+        if (token >= cols) continue;
+        const float s = sum[i] * xs[token];
+        if (sh.slices == 1)
+          put(token, rb * 16 + r, s);
+        else
+          __stcg(mine + token * 16 + r, s);
+      }
     }
     if (sh.slices == 1) continue;
     // the warp (k_split: the CTA's first warps, one after the other) that arrives last at
-    // the row block adds the slices, always in the same order; part: [token group][row
+    // the row block adds the slices, always in the same order; part: [row
     // block][slice][token][16 rows]
     if (split) {
       if (warp * 32 >= cols * 16) continue;
@@ -528,18 +511,18 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
     __syncwarp();
     const uint32_t arrivals = (uint32_t)sh.slices * (split ? (cols * 16 + 31) / 32 : 1);
     uint32_t before = 0;
-    if (lane == 0) before = atomicAdd(a.count + at, 1u);
+    if (lane == 0) before = atomicAdd(a.count + rb, 1u);
     before = __shfl_sync(0xFFFFFFFFu, before, 0);
     if (before != arrivals - 1u) continue;
-    if (lane == 0) a.count[at] = 0u;
+    if (lane == 0) a.count[rb] = 0u;
     __threadfence();
-    const float* all = part + at * sh.slices * (NT * 128);
+    const float* all = part + (int64_t)rb * sh.slices * 128;
     // four rows of one token at a time
     for (int e = lane * 4; e < cols * 16; e += 128) {
       float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
       for (int k = 0; k < sh.slices; ++k) {
-        const float4 p = __ldcg(reinterpret_cast<const float4*>(all + k * (NT * 128) + e));
+        const float4 p = __ldcg(reinterpret_cast<const float4*>(all + k * 128 + e));
         s.x += p.x;
         s.y += p.y;
         s.z += p.z;
@@ -555,20 +538,15 @@ few_linear_kernel(const FewLinearArgs a, const FewShape sh, const uint4* frag, c
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-int few_nt(int64_t T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
-
 FewShape few_shape(int fmt, const FewLinearArgs& a, int sm_count) {
   FewShape s;
-  const int nt = few_nt(a.T), cols = nt == 1 ? (int)a.T : 8 * nt;
+  const int cols = (int)a.T;
   s.steps = (int)((a.kp + few_step(fmt) - 1) / few_step(fmt));
   s.groups = s.steps * few_groups(fmt);
-  s.z = (int)((a.T + 8 * nt - 1) / (8 * nt));
   s.words = a.kp / bf_block(fmt) % 4 == 0 && (reinterpret_cast<uintptr_t>(a.sf) & 3) == 0;
-  s.tile_cols = cols < 8 ? cols : 8;
   // one or two tokens: all of x fits a CTA, whose warps share the row blocks
   s.k_split = a.T <= 2 ? kWarps : 1;
-  // CTAs that run at a time; with several groups of tokens each takes its share
-  const int ctas = (nt <= 4 ? 2 : 1) * sm_count;
+  const int ctas = 2 * sm_count;  // that run at a time
   const int64_t row_blocks = (a.N + 15) / 16, per_cta = kWarps / s.k_split;
   // a part of x has at most 48 KB, and a warp at least two steps of a row block; between
   // these bounds, the cut that leaves the busiest warp the least work
@@ -598,68 +576,53 @@ FewShape few_shape(int fmt, const FewLinearArgs& a, int sm_count) {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t frag_bytes(const FewShape& s, int nt) {
-  return up256((size_t)s.z * s.groups * nt * kPairs * 64 * s.tile_cols);
-}
+size_t frag_bytes(const FewShape& s, int64_t T) { return up256((size_t)s.groups * kPairs * 64 * T); }
 
-template <typename T, int FMT, int NT>
-cudaError_t few_launch(const FewLinearArgs& a, const FewShape& sh, cudaStream_t s) {
+template <typename T, int FMT>
+cudaError_t few_launch(const FewLinearArgs& a, int sm_count, cudaStream_t s) {
+  const FewShape sh = few_shape(FMT, a, sm_count);
   uint4* frag = static_cast<uint4*>(a.ws);
-  float* xs = reinterpret_cast<float*>(static_cast<char*>(a.ws) + frag_bytes(sh, NT));
+  float* xs = reinterpret_cast<float*>(static_cast<char*>(a.ws) + frag_bytes(sh, a.T));
   float* part = xs + up256(a.T * sizeof(float)) / sizeof(float);
-  few_prepare_kernel<T, NT><<<(unsigned)a.T, 512, 0, s>>>(a, sh, frag, xs);
+  few_prepare_kernel<T><<<(unsigned)a.T, 512, 0, s>>>(a, sh, frag, xs);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int smem = sh.x_bytes + kWarps * kAhead * Ring<FMT>::kSlot;
   static std::atomic<int> seen[16];
-  e = allow_smem(few_linear_kernel<T, FMT, NT>, smem, seen);
+  e = allow_smem(few_linear_kernel<T, FMT>, smem, seen);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(sh.slices * sh.rows_ctas), (unsigned)sh.z);
+  cfg.gridDim = dim3((unsigned)(sh.slices * sh.rows_ctas));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, few_linear_kernel<T, FMT, NT>, a, sh,
+  return cudaLaunchKernelEx(&cfg, few_linear_kernel<T, FMT>, a, sh,
                             static_cast<const uint4*>(frag), static_cast<const float*>(xs), part);
-}
-
-template <typename T, int FMT>
-cudaError_t few_nt_launch(const FewLinearArgs& a, int sm_count, cudaStream_t s) {
-  const FewShape sh = few_shape(FMT, a, sm_count);
-  switch (few_nt(a.T)) {
-    case 1: return few_launch<T, FMT, 1>(a, sh, s);
-    case 2: return few_launch<T, FMT, 2>(a, sh, s);
-    case 4: return few_launch<T, FMT, 4>(a, sh, s);
-    default: return few_launch<T, FMT, 8>(a, sh, s);
-  }
 }
 
 template <typename T>
 cudaError_t few_fmt_launch(int fmt, const FewLinearArgs& a, int sm_count, cudaStream_t s) {
-  if (fmt == BF_NVFP4) return few_nt_launch<T, BF_NVFP4>(a, sm_count, s);
-  if (fmt == BF_MXF4) return few_nt_launch<T, BF_MXF4>(a, sm_count, s);
-  return few_nt_launch<T, BF_MXF8>(a, sm_count, s);
+  if (fmt == BF_NVFP4) return few_launch<T, BF_NVFP4>(a, sm_count, s);
+  if (fmt == BF_MXF4) return few_launch<T, BF_MXF4>(a, sm_count, s);
+  return few_launch<T, BF_MXF8>(a, sm_count, s);
 }
 
 }  // namespace
 
 size_t few_linear_ws_bytes(int fmt, const FewLinearArgs& a, int sm_count) {
   const FewShape s = few_shape(fmt, a, sm_count);
-  const int nt = few_nt(a.T);
-  const size_t part = s.slices == 1 ? 0
-                                    : (size_t)s.z * (size_t)((a.N + 15) / 16) * s.slices * nt * 128 *
-                                          sizeof(float);
-  return frag_bytes(s, nt) + up256(a.T * sizeof(float)) + part;
+  const size_t part = s.slices == 1 ? 0 : (size_t)((a.N + 15) / 16) * s.slices * 128 * sizeof(float);
+  return frag_bytes(s, a.T) + up256(a.T * sizeof(float)) + part;
 }
 
 size_t few_linear_counters(int fmt, const FewLinearArgs& a, int sm_count) {
   const FewShape s = few_shape(fmt, a, sm_count);
-  return s.slices > 1 ? (size_t)s.z * (size_t)((a.N + 15) / 16) : 0;
+  return s.slices > 1 ? (size_t)((a.N + 15) / 16) : 0;
 }
 
 cudaError_t launch_few_linear(int fmt, int type, const FewLinearArgs& a, int sm_count,
