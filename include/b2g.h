@@ -541,8 +541,10 @@ B2G_API b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_
 /* out[T][N] = alpha * x[T][K] . W[N][K]^T for the few tokens of a decode step: x and
  * out bf16 or fp16, W as codes and scales in b2g_block_quantize's layout ([N][Kp], Kp =
  * K rounded up to 32, padding zero), x not cast: fp32 sums of products of x and the
- * weights' values.  Reads the weights once for every 64 tokens; for many tokens cast x
- * and use b2g_gemm.  w 16-byte, sfw 2-byte aligned. */
+ * weights' values.  An infinity or a NaN in x makes the outputs of its token infinite or
+ * NaN.  Reads the weights once for every 128 tokens; for many tokens cast x and use
+ * b2g_gemm.  w 16-byte, sfw 2-byte aligned.  From nine tokens on a kernel wait that ran
+ * out is reported by b2g_check, as for b2g_gemm. */
 typedef struct b2g_linear_desc {
   int32_t format;        /* of W */
   int32_t type;          /* of x and out: B2G_BF16 or B2G_F16 */

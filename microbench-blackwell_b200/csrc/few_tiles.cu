@@ -133,46 +133,50 @@ __device__ __forceinline__ bool any_code(int fmt, const uint4& c) {
   return ((c.x | c.y | c.z | c.w) & (fmt == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) != 0u;
 }
 
-// Their products, in fp32 and from global memory, by the thread that decodes them: the part
-// pt of every step of one row, into far[token].  x16: the CTA's first token.
+// The tokens whose sums a decoding thread takes out in the end: 16 of every 64, of one row.
+__device__ __forceinline__ int drained_token(int pt, int j) { return j / 16 * (16 * kParts) + pt * 16 + j % 16; }
+constexpr int kDrained = 128 / kParts;
+
+// The products of a row's blocks that were left out, in fp32 and from global memory, for
+// those tokens: far[j * kDecodeWarps * 32].  x16: the CTA's first token.
 template <int FMT>
 __device__ __noinline__ void far_blocks(const FewLinearArgs& a, const __half* x16, int64_t kq, int row,
-                                        int s0, int s1, int pt, uint32_t ref, int cols, float* far) {
-  constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
-  for (int t = 0; t < cols; ++t) far[t] = 0.0f;
-  const int scales = (int)a.kp / bf_block(FMT);
-  for (int step = s0; step < s1; ++step)
-    for (int p = 0; p < kPieces; ++p) {
-      const int k0 = step * sk + (pt * kPieces + p) * elems;
-      if (k0 >= a.kp) continue;
-      const uint32_t s = __ldg(a.sf + (int64_t)row * scales + k0 / bf_block(FMT));
-      const uint4 c = __ldg(reinterpret_cast<const uint4*>(a.w + ((int64_t)row * a.kp + k0) * bf_bits(FMT) / 8));
-      if (!far_scale<FMT>(s, ref) || !any_code(FMT, c)) continue;
-      for (int t = 0; t < cols; ++t) {
-        float dot = 0.0f;
-        for (int i = 0; i < elems; ++i) {
-          const int at = i * bf_bits(FMT) / 32;
-          const uint32_t word = (at == 0 ? c.x : at == 1 ? c.y : at == 2 ? c.z : c.w) >> (i * bf_bits(FMT) % 32);
-          float v;
-          if constexpr (FMT == BF_MXF8) {
-            v = e4m3_pair(word & 0xFFu).x;
-          } else {
-            uint32_t q[4];
-            e2m1x8_pairs(word & 15u, q);
-            v = __half2float(__ushort_as_half((unsigned short)(q[0] & 0xFFFFu)));
-          }
-          dot = fmaf(v, __half2float(x16[t * kq + k0 + i]), dot);
+                                        int k_begin, int k_end, int pt, uint32_t ref, int cols, float* far) {
+  constexpr int elems = 128 / bf_bits(FMT);
+  for (int j = 0; j < kDrained; ++j) far[j * kDecodeWarps * 32] = 0.0f;
+  const int64_t kp = a.kp;
+  for (int k0 = k_begin; k0 < k_end; k0 += elems) {
+    const uint32_t s = __ldg(a.sf + (row * kp + k0) / bf_block(FMT));
+    if (!far_scale<FMT>(s, ref)) continue;
+    const uint4 c = __ldg(reinterpret_cast<const uint4*>(a.w + (row * kp + k0) * bf_bits(FMT) / 8));
+    if (!any_code(FMT, c)) continue;
+    for (int j = 0; j < kDrained; ++j) {
+      const int t = drained_token(pt, j);
+      if (t >= cols) break;
+      float dot = 0.0f;
+      for (int i = 0; i < elems; ++i) {
+        const int at = i * bf_bits(FMT) / 32;
+        const uint32_t word = (at == 0 ? c.x : at == 1 ? c.y : at == 2 ? c.z : c.w) >> (i * bf_bits(FMT) % 32);
+        float v;
+        if constexpr (FMT == BF_MXF8) {
+          v = e4m3_pair(word & 0xFFu).x;
+        } else {
+          uint32_t q[4];
+          e2m1x8_pairs(word & 15u, q);
+          v = __half2float(__ushort_as_half((unsigned short)(q[0] & 0xFFFFu)));
         }
-        far[t] = fmaf(e8m0_value(s), dot, far[t]);
+        dot = fmaf(v, __half2float(x16[t * kq + k0 + i]), dot);
       }
+      far[j * kDecodeWarps * 32] = fmaf(e8m0_value(s), dot, far[j * kDecodeWarps * 32]);
     }
+  }
 }
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads, 1)
 few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                  const FewLinearArgs a, const TileShape sh, const __half* x16, const float* xs,
-                 float* part, float* far_ws) {
+                 float* part) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // ring slots (codes, x, scales) start on 1024 bytes
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -180,7 +184,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
   __shared__ bool last;
-  __shared__ float ref_scale[kRows];
+  __shared__ uint8_t row_ref[kRows];
   __shared__ uint8_t has_far[kParts][kRows];
   constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
   constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
@@ -322,7 +326,6 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     constexpr int per_step = sk / bf_block(FMT);
     const uint8_t* sf = a.sf + (int64_t)row * scales;
     uint32_t ref = 0;
-    float* far = nullptr;
     if constexpr (FMT != BF_NVFP4) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -334,8 +337,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           ref = s > ref && s != 255u ? s : ref;  // a NaN scale says nothing of the others
         }
       }
-      if (pt == 0) ref_scale[r] = e8m0_value(ref);
-      far = far_ws + ((((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kParts + pt) * kRows + r) * 128;
+      if (pt == 0) row_ref[r] = (uint8_t)ref;
     }
     int stage = 0;
     uint32_t round = 0;
@@ -424,26 +426,33 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         round ^= 1u;
       }
     }
-    if constexpr (FMT != BF_NVFP4) {
-      has_far[pt][r] = any_far;
-      // x has been read through the ring, so the kernel that laid it out has ended
-      if (any_far && !aborted)
-        far_blocks<FMT>(a, x16 + (int64_t)token0 * sh.steps * sk, (int64_t)sh.steps * sk, row, s0, s1, pt,
-                        ref, cols, far);
-    }
+    if constexpr (FMT != BF_NVFP4) has_far[pt][r] = any_far;
   }
 
   tc_fence_before();
-  __syncthreads();  // the products are done (their warp waited for them)
+  __syncthreads();  // the products are done and the copies landed (their warps waited for them)
   tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // over long since: xs and x16 are read below
   const int n = (int)a.N;
   const int64_t at = (int64_t)blockIdx.y * sh.row_tiles + tile;
   float* mine = part + (at * sh.slices + slice) * ((int64_t)sh.tokens * kRows);
   if (warp < kDecodeWarps && !aborted) {
     const int pt = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float scale = FMT == BF_NVFP4 ? 1.0f : ref_scale[r];
-    const float* f0 = far_ws + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kParts * kRows + r) * 128;
+    float scale = 1.0f;
+    bool any_far = false;
+    // the ring is free: 64 KB of it for 32 tokens a thread
+    float* far = static_cast<float*>(__cvta_shared_to_generic(ring)) + threadIdx.x;
+    if constexpr (FMT != BF_NVFP4) {
+      scale = e8m0_value(row_ref[r]);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) any_far |= has_far[q][r] != 0;
+      if (any_far)
+        far_blocks<FMT>(a, x16 + (int64_t)token0 * sh.steps * sk, (int64_t)sh.steps * sk,
+                        row0 + r < n ? row0 + r : n - 1, s0 * sk, min(s1 * sk, (int)a.kp), pt, row_ref[r],
+                        cols, far);
+      __syncwarp();
+    }
     for (int c = pt * 16; c < sh.tokens; c += 16 * kParts) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + lanes + c, v);
@@ -455,9 +464,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         const float d = __uint_as_float(v[i]);
         float sum = FMT == BF_NVFP4 || d == 0.0f ? d : d * scale;
         if constexpr (FMT != BF_NVFP4) {
-#pragma unroll
-          for (int q = 0; q < kParts; ++q)
-            if (has_far[q][r]) sum += __ldcg(f0 + q * (kRows * 128) + t);
+          if (any_far) sum += far[(c / (16 * kParts) * 16 + i) * kDecodeWarps * 32];
         }
         if (sh.slices > 1)
           __stcg(mine + t * kRows + r, sum);
@@ -529,16 +536,15 @@ TileShape tile_shape(int fmt, const FewLinearArgs& a, int sm_count) {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct TileWs {
-  size_t x16, xs, far, part, total;
+  size_t x16, xs, part, total;
 };
 
 TileWs tile_ws(int fmt, const FewLinearArgs& a, const TileShape& s) {
   TileWs w;
   w.x16 = 0;
   w.xs = up256((size_t)a.T * s.steps * step_k(fmt) * 2);
-  w.far = w.xs + up256((size_t)a.T * sizeof(float));
+  w.part = w.xs + up256((size_t)a.T * sizeof(float));
   const size_t ctas = (size_t)s.row_tiles * s.slices * s.z;
-  w.part = w.far + (fmt == BF_NVFP4 ? 0 : ctas * kParts * kRows * 128 * sizeof(float));
   w.total = w.part + (s.slices > 1 ? ctas * s.tokens * kRows * sizeof(float) : 0);
   return w;
 }
@@ -567,7 +573,7 @@ cudaError_t tiles_launch(const FewLinearArgs& a, const TileShape& sh, const CUte
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, few_tiles_kernel<T, FMT>, mw, mx, a, sh,
                             reinterpret_cast<const __half*>(ws + w.x16), static_cast<const float*>(xs),
-                            reinterpret_cast<float*>(ws + w.part), reinterpret_cast<float*>(ws + w.far));
+                            reinterpret_cast<float*>(ws + w.part));
 }
 
 }  // namespace

@@ -615,6 +615,145 @@ def test_no_tokens(engine):
                   torch.empty(0, 16, dtype=torch.bfloat16, device="cuda"), FMT["nvfp4"])
 
 
+# ------------------------------------------------------------------ tens of tokens
+@pytest.mark.parametrize("fmt", ["mxf4", "mxf8"])
+@pytest.mark.parametrize("T,N,K", [(9, 40, 512), (70, 131, 352), (130, 20, 2400)])
+def test_tens_of_tokens_with_scales_far_apart(engine, fmt, T, N, K):
+    # blocks outside fp16's range of their row's reference, here and there or nearly all
+    rng = np.random.default_rng(T)
+    for lo, hi in ((90, 160), (112, 134)):
+        codes, sf, w = random_weights(fmt, N, K, 51 + lo, lo, hi)
+        block_max = 2.0 ** (sf[:, :K // 32].astype(float).mean(0) - 127)
+        x = rounded(rng.normal(size=(T, K)) / np.repeat(block_max, 32) ** 0.5, "bf16")
+        check_linear(engine, x, codes, sf, w, fmt, "bf16")
+    # one block that counts, behind far larger scales on blocks of zeros
+    codes[:, :] = 0
+    sf[:, :] = 200
+    codes[:, 0] = 0x22 if fmt == "mxf4" else 0x38
+    sf[:, 0] = 100
+    check_linear(engine, x, codes, sf, ref.values(codes, sf, fmt)[:, :K], fmt, "bf16")
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+def test_tens_of_tokens_with_x_of_a_wide_range(engine, fmt):
+    T, N, K = 20, 64, 256
+    rng = np.random.default_rng(52)
+    x = rng.normal(size=(T, K)) * 2.0 ** rng.integers(-60, 60, size=(T, K))
+    x[1] *= 2.0 ** -60
+    x[2] = 0
+    codes, sf, w = random_weights(fmt, N, K, 53)
+    check_linear(engine, rounded(x, "bf16"), codes, sf, w, fmt, "bf16", alpha=2.0 ** -20)
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("T", [3, 12])
+def test_products_of_infinities_and_nan(engine, fmt, T):
+    N, K = 150, 320
+    codes, sf, w = random_weights(fmt, N, K, 54)
+    x = rounded(np.random.default_rng(55).normal(size=(T, K)) / 64, "bf16")
+    x[1, 300], x[2, 9] = -np.inf, np.nan
+    c, s = torch.from_numpy(codes).cuda(), torch.from_numpy(sf).cuda()
+    out = torch.empty(T, N, dtype=torch.bfloat16, device="cuda")
+    engine.linear(dev(x, torch.bfloat16), c, s, out, FMT[fmt])
+    got = host(out)
+    assert np.isfinite(np.delete(got, (1, 2), 0)).all() and np.isnan(got[2]).all()
+    some = w[:, 300] != 0
+    assert np.array_equal(got[1][some], np.sign(w[some, 300]) * -np.inf) and np.isnan(got[1][~some]).all()
+    # a NaN scale reaches the outputs of its row alone, where it is a row's first, and its last
+    x[1, 300] = x[2, 9] = 0
+    s[5, 0] = s[140, -1] = 127 if fmt == "nvfp4" else 255
+    engine.linear(dev(x, torch.bfloat16), c, s, out, FMT[fmt])
+    got = host(out)
+    assert np.isnan(got[:, [5, 140]]).all() and np.isfinite(np.delete(got, (5, 140), 1)).all()
+    # with blocks that are left out of the tensor product an infinity may become a NaN, not a number
+    if fmt != "nvfp4":
+        codes, sf, _ = random_weights(fmt, N, K, 56, 60, 190)
+        x[0, 40] = np.inf
+        engine.linear(dev(x, torch.bfloat16), torch.from_numpy(codes).cuda(), torch.from_numpy(sf).cuda(), out,
+                      FMT[fmt])
+        got = host(out)
+        assert not np.isfinite(got[0]).any() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("T", [5, 24])
+def test_weights_and_scales_at_odd_places(engine, fmt, T):
+    # codes on 16 bytes, scales on two, neither on the allocation's start
+    N, K = 70, 1120
+    codes, sf, w = random_weights(fmt, N, K, 57)
+    c = torch.zeros(codes.size + 16, dtype=torch.uint8, device="cuda")[16:].view(codes.shape)
+    s = torch.zeros(sf.size + 2, dtype=torch.uint8, device="cuda")[2:].view(sf.shape)
+    c.copy_(torch.from_numpy(codes)), s.copy_(torch.from_numpy(sf))
+    x = dev(np.random.default_rng(58).normal(size=(T, K)), torch.float16, 3)
+    here, there = (torch.empty(T, N, dtype=torch.float16, device="cuda") for _ in range(2))
+    engine.linear(x, c, s, here, FMT[fmt], alpha=1 / 64)
+    engine.linear(x, torch.from_numpy(codes).cuda(), torch.from_numpy(sf).cuda(), there, FMT[fmt], alpha=1 / 64)
+    assert torch.equal(here, there) and torch.isfinite(here).all()
+
+
+def test_tens_of_tokens_repeat_to_the_bit_on_another_stream_and_in_a_graph(engine):
+    codes, sf, _ = random_weights("mxf8", 300, 8192, 59)
+    c, s = torch.from_numpy(codes).cuda(), torch.from_numpy(sf).cuda()
+    x = dev(np.random.default_rng(60).normal(size=(40, 8192)) / 64, torch.bfloat16)
+    first, out = (torch.empty(40, 300, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    engine.linear(x, c, s, first, FMT["mxf8"])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    engine.linear(x, c, s, out, FMT["mxf8"], stream=side)
+    side.synchronize()
+    assert torch.equal(first, out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        engine.linear(x, c, s, out, FMT["mxf8"])
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, out)
+    engine.check()
+
+
+@pytest.mark.parametrize("typ", list(TYPE))
+@pytest.mark.parametrize("cols", [1, 2, 7, 9, 15, 17, 31, 257])
+def test_norm_passes_of_narrow_rows_at_odd_places(engine, typ, cols):
+    # the words that hold a row's ends may hold its neighbours' too, and what lies outside
+    rows, per = 9, 2
+    a = norm_case(typ, rows, cols, per, 61 + cols)
+    v, h, r1, r2 = ref.norm_forward(**a, per=per)
+    dt = TYPE[typ]
+
+    def odd(m):  # contiguous, one element behind an aligned place
+        flat = torch.full((m.size + 2,), float("nan"), dtype=dt, device="cuda")
+        flat[1:-1] = torch.as_tensor(m.reshape(-1)).to(dt)
+        return flat, flat[1:-1].view(m.shape)
+
+    t = {k: odd(m)[1] for k, m in a.items()}
+    t["w_pre"], t["w_post"] = t["w_pre"].view(-1), t["w_post"].view(-1)
+    xo, ho, dx, dy = (odd(np.zeros((rows, cols))) for _ in range(4))
+    s1, s2 = (torch.empty(rows, device="cuda") for _ in range(2))
+    engine.residual_norm(t["x"], y=t["y"], gate=t["gate"], rows_per_gate=per, w_post=t["w_post"],
+                         w_pre=t["w_pre"], x_out=xo[1], h=ho[1], rstd_post=s1, rstd_pre=s2)
+    bx, (_, bh) = norm_bounds(a, per, v, h, r2, 1.0, 1.0, typ, cols)
+    assert np.all(np.abs(host(xo[1]) - v) <= bx) and np.all(np.abs(host(ho[1]) - h) <= bh)
+
+    rng = np.random.default_rng(cols)
+    dh, dxo, v = (rounded(rng.normal(size=(rows, cols)), typ) for _ in range(3))
+    r1, r2 = (rounded(1 / np.sqrt((m * m).mean(1) + 1e-6), "f32") for m in (a["y"], v))
+    want = ref.norm_backward(dh, dxo, v, r2, a["w_pre"], a["y"], r1, a["w_post"], a["gate"], per, 1.0, 1.0)
+    out = {k: torch.empty(want[k].shape, device="cuda") for k in ("dgate", "dw_post", "dw_pre")}
+    engine.residual_norm_backward(
+        odd(dh)[1], odd(v)[1], torch.as_tensor(r2).float().cuda(), t["w_pre"], dx[1], dx_out=odd(dxo)[1],
+        y=t["y"], rstd_post=torch.as_tensor(r1).float().cuda(), w_post=t["w_post"], gate=t["gate"],
+        rows_per_gate=per, dy=dy[1], **out)
+    out.update(dx=dx[1], dy=dy[1])
+    for k, b in grad_bounds(a, v, dh, dxo, r1, r2, per, 1.0, 1.0, typ, cols, rows).items():
+        if k in ("dx", "dy"):
+            b = b + ULP[typ] * (np.abs(want[k]) + b) + TINY[typ]
+        assert np.all(np.abs(host(out[k]) - want[k]) <= b + 1e-37), k
+    for flat, _ in (xo, ho, dx, dy):
+        assert torch.isnan(flat[[0, -1]]).all()
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(engine):
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
