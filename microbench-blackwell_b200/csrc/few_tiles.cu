@@ -109,13 +109,12 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A thread's scale bytes of a part: NVFP4 4, MXFP4 2, MXFP8 1; zeros past the row's end.
-template <int FMT>
+// N scale bytes of a row of `count`; zeros past its end.
+template <int N>
 __device__ __forceinline__ uint32_t load_scales(const uint8_t* row, int first, int count) {
-  constexpr int n = step_k(FMT) / kParts / bf_block(FMT);
   uint32_t s = 0u;
 #pragma unroll
-  for (int i = 0; i < n; ++i) s |= (first + i < count ? (uint32_t)__ldg(row + first + i) : 0u) << (8 * i);
+  for (int i = 0; i < N; ++i) s |= (first + i < count ? (uint32_t)__ldg(row + first + i) : 0u) << (8 * i);
   return s;
 }
 
@@ -184,7 +183,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
   __shared__ bool last;
-  __shared__ uint8_t row_ref[kRows];
+  __shared__ uint32_t row_ref[kRows];
   __shared__ uint8_t has_far[kParts][kRows];
   constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
   constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
@@ -201,6 +200,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   auto a_empty = [&](int b) { return smem_u32(&bars[2 * kMaxStages + 2 + b]); };
   const uint32_t done = smem_u32(&bars[2 * kMaxStages + 4]);
 
+  if (threadIdx.x < kRows) row_ref[threadIdx.x] = 0u;
   if (threadIdx.x == 0) {
     aborted = 0;
     for (int s = 0; s < kMaxStages; ++s) {
@@ -327,17 +327,32 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint8_t* sf = a.sf + (int64_t)row * scales;
     uint32_t ref = 0;
     if constexpr (FMT != BF_NVFP4) {
+      // the largest scale of eight steps spread over the slice, two of them a part's; a NaN
+      // scale says nothing of the others
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int step = s0 + (s1 - s0) * q / 8;
-        const uint32_t w = load_scales<FMT>(sf, step * per_step, scales);
+      for (int q = 2 * pt; q < 2 * pt + 2; ++q) {
+        const int first = (s0 + (s1 - s0) * q / 8) * per_step;
+        uint32_t w[per_step / 4];
+        if (sh.words) {
+          if constexpr (per_step == 8) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(sf + first));
+            w[0] = v.x, w[1] = v.y;
+          } else {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(sf + first));
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < per_step / kParts; ++i) {
-          const uint32_t s = (w >> (8 * i)) & 0xFFu;
-          ref = s > ref && s != 255u ? s : ref;  // a NaN scale says nothing of the others
+          for (int i = 0; i < per_step / 4; ++i) w[i] = load_scales<4>(sf, first + 4 * i, scales);
+        }
+#pragma unroll
+        for (int i = 0; i < per_step; ++i) {
+          const uint32_t s = (w[i / 4] >> (8 * (i % 4))) & 0xFFu;
+          ref = s > ref && s != 255u ? s : ref;
         }
       }
-      if (pt == 0) row_ref[r] = (uint8_t)ref;
+      atomicMax(&row_ref[r], ref);
+      asm volatile("bar.sync 1, %0;" ::"n"(kDecodeWarps * 32) : "memory");
+      ref = row_ref[r];
     }
     int stage = 0;
     uint32_t round = 0;
@@ -365,7 +380,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           asm volatile("ld.shared.u8 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
         }
       } else {
-        now = load_scales<FMT>(sf, (s0 + i) * per_step + pt * mine_n, scales);
+        now = load_scales<mine_n>(sf, (s0 + i) * per_step + pt * mine_n, scales);
       }
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
