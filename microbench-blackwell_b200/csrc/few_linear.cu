@@ -299,6 +299,10 @@ struct FewShape {
 // covers the memory's latency at its rate.
 constexpr int kAhead = 4;
 
+// Bytes of x in a CTA: with the warps' rings (up to 72 KB) and their sums (8 KB) two CTAs fit
+// an SM.
+constexpr int kMaxX = 32768;
+
 // x as fp16 B fragments: [group][step pair][4 threads][token] of 16 bytes, the four
 // elements of two steps; xs[token] = the power of two to undo.  Of eight tokens column c of thread t and pair jp lies at c ^ (jp + 4 (t % 2)): the lanes that
 // read it, and the eight neighbours that write one column, meet different banks.  Zero past
@@ -544,14 +548,14 @@ FewShape few_shape(int fmt, const FewLinearArgs& a, int sm_count) {
   s.steps = (int)((a.kp + few_step(fmt) - 1) / few_step(fmt));
   s.groups = s.steps * few_groups(fmt);
   s.words = a.kp / bf_block(fmt) % 4 == 0 && (reinterpret_cast<uintptr_t>(a.sf) & 3) == 0;
-  // one or two tokens: all of x fits a CTA, whose warps share the row blocks
-  s.k_split = a.T <= 2 ? kWarps : 1;
+  // all of x in a CTA: its warps share the row blocks
+  const int64_t x_all = (int64_t)s.groups * cols * kGroup * 2;
+  s.k_split = x_all <= kMaxX ? kWarps : 1;
   const int ctas = 2 * sm_count;  // that run at a time
   const int64_t row_blocks = (a.N + 15) / 16, per_cta = kWarps / s.k_split;
-  // a part of x has at most 48 KB, and a warp at least two steps of a row block; between
-  // these bounds, the cut that leaves the busiest warp the least work
-  int least = (int)(((int64_t)s.groups * cols * kGroup * 2 + 49151) / 49152);
-  least = least < 1 ? 1 : least;
+  // a warp has at least two steps of a row block; between the bounds, the cut that leaves
+  // the busiest warp the least work
+  const int least = (int)((x_all + kMaxX - 1) / kMaxX);
   const int most = s.steps / (2 * s.k_split) > least ? s.steps / (2 * s.k_split) : least;
   int64_t best = INT64_MAX;
   s.slices = least;
