@@ -20,12 +20,15 @@ namespace b2g {
 namespace {
 
 constexpr int kRows = 128;            // weight rows of a CTA
-constexpr int kParts = 4;             // of a step, each decoded by four warps
-constexpr int kDecodeWarps = 4 * kParts;
-constexpr int kPieces = 8 / kParts;   // 16-byte pieces of a row in a part
+// Two groups of eight decoding warps take every other step each; four of them cover the rows,
+// twice, for the halves of a step.
+constexpr int kGroups = 2, kHalves = 2;
+constexpr int kQuads = kGroups * kHalves;  // sets of four warps
+constexpr int kDecodeWarps = 4 * kQuads;
 constexpr int kThreads = (kDecodeWarps + 2) * 32;
 constexpr int kCodeBytes = 128;       // of a row in a step
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 6;
+constexpr int kMaxBuffers = 4;
 constexpr int kScaleBytes = 2048;     // of a ring slot: 16, 8 or 4 bytes a row
 
 __host__ __device__ constexpr int step_k(int fmt) { return kCodeBytes * 8 / bf_bits(fmt); }
@@ -123,39 +126,35 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* row, int first, i
 // - ref from -14 to 13 (e2m1) or 7 (e4m3).  Blocks outside (and not all zeros) are left out
 // of the tensor product.
 template <int FMT>
-__device__ __forceinline__ bool far_scale(uint32_t s, uint32_t ref) {
-  const int d = (int)s - (int)ref;
-  return s != 255u && (d < -14 || d > (FMT == BF_MXF8 ? 7 : 13));
+constexpr uint32_t kAbove = FMT == BF_MXF8 ? 7 : 13;
+
+template <int FMT>
+__device__ __forceinline__ bool any_code(const uint32_t (&c)[bf_bits(FMT)]) {
+  uint32_t any = 0u;
+#pragma unroll
+  for (int i = 0; i < bf_bits(FMT); ++i) any |= c[i];
+  return (any & (FMT == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) != 0u;
 }
 
-__device__ __forceinline__ bool any_code(int fmt, const uint4& c) {
-  return ((c.x | c.y | c.z | c.w) & (fmt == BF_MXF8 ? 0x7F7F7F7Fu : 0x77777777u)) != 0u;
-}
-
-// The tokens whose sums a decoding thread takes out in the end: 16 of every 64, of one row.
-__device__ __forceinline__ int drained_token(int pt, int j) { return j / 16 * (16 * kParts) + pt * 16 + j % 16; }
-constexpr int kDrained = 128 / kParts;
-
-// The products of a row's blocks that were left out, in fp32 and from global memory, for
-// those tokens: far[j * kDecodeWarps * 32].  x16: the CTA's first token.
+// The products of a row's blocks that were left out, in fp32 and from global memory:
+// far[j * kDecodeWarps * 32] of the j-th of `count` tokens, whose x starts at x16.
 template <int FMT>
 __device__ __noinline__ void far_blocks(const FewLinearArgs& a, const __half* x16, int64_t kq, int row,
-                                        int k_begin, int k_end, int pt, uint32_t ref, int cols, float* far) {
-  constexpr int elems = 128 / bf_bits(FMT);
-  for (int j = 0; j < kDrained; ++j) far[j * kDecodeWarps * 32] = 0.0f;
+                                        int k_begin, int k_end, uint32_t ref, int count, float* far) {
+  for (int j = 0; j < count; ++j) far[j * kDecodeWarps * 32] = 0.0f;
   const int64_t kp = a.kp;
-  for (int k0 = k_begin; k0 < k_end; k0 += elems) {
-    const uint32_t s = __ldg(a.sf + (row * kp + k0) / bf_block(FMT));
-    if (!far_scale<FMT>(s, ref)) continue;
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(a.w + (row * kp + k0) * bf_bits(FMT) / 8));
-    if (!any_code(FMT, c)) continue;
-    for (int j = 0; j < kDrained; ++j) {
-      const int t = drained_token(pt, j);
-      if (t >= cols) break;
+  for (int k0 = k_begin; k0 < k_end; k0 += 32) {
+    const uint32_t s = __ldg(a.sf + (row * kp + k0) / 32);
+    if (s == 255u || s - ref + 14u <= 14u + kAbove<FMT>) continue;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.w + (row * kp + k0) * bf_bits(FMT) / 8);
+    uint32_t c[bf_bits(FMT)];
+    for (int i = 0; i < bf_bits(FMT); ++i) c[i] = __ldg(codes + i);
+    if (!any_code<FMT>(c)) continue;
+    for (int j = 0; j < count; ++j) {
+      const __half* x = x16 + j * kq + k0;
       float dot = 0.0f;
-      for (int i = 0; i < elems; ++i) {
-        const int at = i * bf_bits(FMT) / 32;
-        const uint32_t word = (at == 0 ? c.x : at == 1 ? c.y : at == 2 ? c.z : c.w) >> (i * bf_bits(FMT) % 32);
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t word = __ldg(codes + i * bf_bits(FMT) / 32) >> (i * bf_bits(FMT) % 32);
         float v;
         if constexpr (FMT == BF_MXF8) {
           v = e4m3_pair(word & 0xFFu).x;
@@ -164,7 +163,7 @@ __device__ __noinline__ void far_blocks(const FewLinearArgs& a, const __half* x1
           e2m1x8_pairs(word & 15u, q);
           v = __half2float(__ushort_as_half((unsigned short)(q[0] & 0xFFFFu)));
         }
-        dot = fmaf(v, __half2float(x16[t * kq + k0 + i]), dot);
+        dot = fmaf(v, __half2float(x[i]), dot);
       }
       far[j * kDecodeWarps * 32] = fmaf(e8m0_value(s), dot, far[j * kDecodeWarps * 32]);
     }
@@ -179,14 +178,17 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // ring slots (codes, x, scales) start on 1024 bytes
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4 + 1];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBuffers + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int aborted;
   __shared__ bool last;
   __shared__ uint32_t row_ref[kRows];
-  __shared__ uint8_t has_far[kParts][kRows];
-  constexpr int sk = step_k(FMT), elems = 128 / bf_bits(FMT);
+  __shared__ float token_scale[128];
+  __shared__ uint8_t has_far[kQuads][kRows];
+  constexpr int sk = step_k(FMT);
   constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
+  constexpr int buffers = FMT == BF_MXF8 ? 4 : 3;   // of them
+  static_assert(buffers <= kMaxBuffers && 128 + buffers * a_cols <= 512, "tensor memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = (int)blockIdx.x / sh.slices, slice = (int)blockIdx.x % sh.slices;
   const int s0 = (int)((unsigned)sh.steps * (unsigned)slice / (unsigned)sh.slices);
@@ -197,8 +199,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   auto full = [&](int s) { return smem_u32(&bars[s]); };
   auto empty = [&](int s) { return smem_u32(&bars[kMaxStages + s]); };
   auto a_full = [&](int b) { return smem_u32(&bars[2 * kMaxStages + b]); };
-  auto a_empty = [&](int b) { return smem_u32(&bars[2 * kMaxStages + 2 + b]); };
-  const uint32_t done = smem_u32(&bars[2 * kMaxStages + 4]);
+  auto a_empty = [&](int b) { return smem_u32(&bars[2 * kMaxStages + kMaxBuffers + b]); };
+  const uint32_t done = smem_u32(&bars[2 * kMaxStages + 2 * kMaxBuffers]);
 
   if (threadIdx.x < kRows) row_ref[threadIdx.x] = 0u;
   if (threadIdx.x == 0) {
@@ -207,8 +209,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       mbar_init(full(s), 1 + 32);  // the copies' byte count, and a lane's scales each
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(a_full(b), kDecodeWarps);
+    for (int b = 0; b < buffers; ++b) {
+      mbar_init(a_full(b), 4 * kHalves);
       mbar_init(a_empty(b), 1);
     }
     mbar_init(done, 1);
@@ -221,7 +223,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot, tmem_a = tmem + 128;  // sums, then two decoded steps
+  const uint32_t tmem = tmem_slot, tmem_a = tmem + 128;  // sums, then decoded steps
 
   if (warp == kDecodeWarps + 1) {
     // ---- copies: codes and scales at once, x when the first kernel has laid it out
@@ -286,12 +288,11 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     // ---- products
     const uint32_t idesc = encode_idesc(KIND_F16, 0, 0, 128, sh.tokens, 0, 0);
     const uint32_t on = elect_one() ? 1u : 0u;
-    int stage = 0;
-    uint32_t round = 0;
+    int stage = 0, b = 0;
+    uint32_t round = 0, turn = 0;
     for (int i = 0; i < s1 - s0; ++i) {
-      const int b = i & 1;
       bool ok = mbar_wait(full(stage), round, &aborted, a.err, ERRW_TIMEOUT_MMA, a.wait_ns);
-      ok = ok && mbar_wait(a_full(b), (uint32_t)(i >> 1) & 1u, &aborted, a.err, ERRW_TIMEOUT_MMA, a.wait_ns);
+      ok = ok && mbar_wait(a_full(b), turn, &aborted, a.err, ERRW_TIMEOUT_MMA, a.wait_ns);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -304,6 +305,10 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       tc_commit<1>(a_empty(b), on);
       tc_commit<1>(empty(stage), on);
       __syncwarp();
+      if (++b == buffers) {
+        b = 0;
+        turn ^= 1u;
+      }
       if (++stage == sh.stages) {
         stage = 0;
         round ^= 1u;
@@ -318,8 +323,8 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     }
     __syncwarp();
   } else {
-    // ---- decoding: row `r`, part `pt` of each step
-    const int pt = warp >> 2, r = (warp & 3) * 32 + lane;
+    // ---- decoding: row `r`, one half of every other step
+    const int quad = warp >> 2, group = quad / kHalves, half = quad % kHalves, r = (warp & 3) * 32 + lane;
     const int row = row0 + r < (int)a.N ? row0 + r : (int)a.N - 1;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int scales = (int)a.kp / bf_block(FMT);             // of a row
@@ -327,10 +332,10 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     const uint8_t* sf = a.sf + (int64_t)row * scales;
     uint32_t ref = 0;
     if constexpr (FMT != BF_NVFP4) {
-      // the largest scale of eight steps spread over the slice, two of them a part's; a NaN
+      // the largest scale of eight steps spread over the slice, two of them a quad's; a NaN
       // scale says nothing of the others
 #pragma unroll
-      for (int q = 2 * pt; q < 2 * pt + 2; ++q) {
+      for (int q = 2 * quad; q < 2 * quad + 2; ++q) {
         const int first = (s0 + (s1 - s0) * q / 8) * per_step;
         uint32_t w[per_step / 4];
         if (sh.words) {
@@ -354,63 +359,67 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       asm volatile("bar.sync 1, %0;" ::"n"(kDecodeWarps * 32) : "memory");
       ref = row_ref[r];
     }
-    int stage = 0;
-    uint32_t round = 0;
+    int stage = group, b = group;
+    uint32_t round = 0, turn = 1;
     bool any_far = false;
-    constexpr int mine_n = per_step / kParts;  // scale bytes of a part
-    for (int i = 0; i < s1 - s0; ++i) {
-      const int b = i & 1;
+    constexpr int mine_n = per_step / kHalves;  // scale bytes of a half: 8, 4 or 2
+    constexpr int units = sk / kHalves / 32;    // of 32 elements
+    const uint32_t to0 = tmem_a + lanes + half * (units * 16);
+    for (int i = group; i < s1 - s0; i += kGroups) {
       bool ok = mbar_wait(full(stage), round, &aborted, a.err, ERRW_TIMEOUT_OTHER, a.wait_ns);
-      ok = ok && (i < 2 || mbar_wait(a_empty(b), (uint32_t)((i >> 1) - 1) & 1u, &aborted, a.err,
-                                     ERRW_TIMEOUT_OTHER, a.wait_ns));
+      ok = ok && (i < buffers || mbar_wait(a_empty(b), turn, &aborted, a.err, ERRW_TIMEOUT_OTHER, a.wait_ns));
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t slot = ring + stage * slot_bytes;
-      uint32_t now;
+      const uint32_t slot = ring + stage * slot_bytes, to = to0 + b * a_cols;
+      uint32_t now[2] = {0u, 0u};
       if (sh.words) {
-        const uint32_t at = slot + kRows * kCodeBytes + x_bytes + r * per_step + pt * mine_n;
-        if constexpr (mine_n == 4) {
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
-        } else if constexpr (mine_n == 2) {
+        const uint32_t at = slot + kRows * kCodeBytes + x_bytes + r * per_step + half * mine_n;
+        if constexpr (mine_n == 8) {
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(now[0]), "=r"(now[1]) : "r"(at) : "memory");
+        } else if constexpr (mine_n == 4) {
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(now[0]) : "r"(at) : "memory");
+        } else {
           uint16_t h;
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at) : "memory");
-          now = h;
-        } else {
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
+          now[0] = h;
         }
       } else {
-        now = load_scales<mine_n>(sf, (s0 + i) * per_step + pt * mine_n, scales);
+        const int first = (s0 + i) * per_step + half * mine_n;
+#pragma unroll
+        for (int k = 0; k < (mine_n + 3) / 4; ++k)
+          now[k] = load_scales<mine_n < 4 ? mine_n : 4>(sf, first + 4 * k, scales);
       }
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        const int piece = pt * kPieces + p;
-        uint32_t c[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-                     : "r"(slot + r * kCodeBytes + ((piece ^ (r & 7)) << 4))
-                     : "memory");
-        // multipliers of the piece's halves
+      for (int u = 0; u < units; ++u) {
+        constexpr int pieces = bf_bits(FMT) / 4;  // of 16 bytes in a unit
+        uint32_t c[4 * pieces];
+#pragma unroll
+        for (int p = 0; p < pieces; ++p)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(c[4 * p]), "=r"(c[4 * p + 1]), "=r"(c[4 * p + 2]), "=r"(c[4 * p + 3])
+                       : "r"(slot + r * kCodeBytes + ((((half * units + u) * pieces + p) ^ (r & 7)) << 4))
+                       : "memory");
+        // multipliers of the unit's halves
         uint32_t m[2];
         if constexpr (FMT == BF_NVFP4) {
           uint32_t h;
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(now >> (16 * p))));
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(now[u / 2] >> (16 * (u % 2)))));
           m[0] = __byte_perm(h, 0, 0x1010);
           m[1] = __byte_perm(h, 0, 0x3232);
         } else {
-          // a block is two 16-byte pieces of 8-bit codes, one of 4-bit codes
-          const uint32_t s = (now >> (8 * (FMT == BF_MXF8 ? p / 2 : p))) & 0xFFu;
-          m[0] = s == 255u ? 0x7E007E00u : (uint32_t)((int)s - (int)ref + 15) * 0x04000400u;
-          if (far_scale<FMT>(s, ref)) {
-            m[0] = 0u;
-            any_far |= any_code(FMT, make_uint4(c[0], c[1], c[2], c[3]));
+          const uint32_t s = (now[0] >> (8 * u)) & 0xFFu, e = s - ref + 15u;  // fp16's exponent
+          m[0] = e * 0x04000400u;
+          if (e - 1u > 14u + kAbove<FMT> || s == 255u) {
+            m[0] = s == 255u ? 0x7E007E00u : 0u;
+            any_far |= s != 255u && any_code<FMT>(c);
           }
           m[1] = m[0];
         }
-        uint32_t f[elems / 2];
+        uint32_t f[16];
         if constexpr (FMT == BF_MXF8) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 16; ++k) {
             asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f[k]) : "h"((uint16_t)(c[k >> 1] >> (16 * (k & 1)))));
             f[k] = mul_h2(f[k], m[0]);
           }
@@ -423,37 +432,39 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             for (int j = 0; j < 4; ++j) f[4 * k + j] = mul_h2(q[j], m[k >> 1]);
           }
         }
-        const uint32_t to = tmem_a + b * a_cols + lanes + piece * (elems / 2);
-        if constexpr (FMT == BF_MXF8) {
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(to),
-                       "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]), "r"(f[4]), "r"(f[5]), "r"(f[6]), "r"(f[7])
-                       : "memory");
-        } else {
-          tmem_st_32x32b_x16(to, f);
-        }
+        __syncwarp();
+        tmem_st_32x32b_x16(to + u * 16, f);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(a_full(b));
-      if (++stage == sh.stages) {
-        stage = 0;
+      b += kGroups;
+      if (b >= buffers) {
+        b -= buffers;
+        turn ^= 1u;
+      }
+      stage += kGroups;
+      if (stage >= sh.stages) {
+        stage -= sh.stages;
         round ^= 1u;
       }
     }
-    if constexpr (FMT != BF_NVFP4) has_far[pt][r] = any_far;
+    if constexpr (FMT != BF_NVFP4) has_far[quad][r] = any_far;
   }
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // over long since: xs and x16 are read now
+  if (threadIdx.x < cols) token_scale[threadIdx.x] = __ldcg(xs + token0 + threadIdx.x);
   tc_fence_before();
   __syncthreads();  // the products are done and the copies landed (their warps waited for them)
   tc_fence_after();
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // over long since: xs and x16 are read below
   const int n = (int)a.N;
   const int64_t at = (int64_t)blockIdx.y * sh.row_tiles + tile;
   float* mine = part + (at * sh.slices + slice) * ((int64_t)sh.tokens * kRows);
   if (warp < kDecodeWarps && !aborted) {
-    const int pt = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int quad = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int first = quad * (sh.tokens / kQuads);  // of this thread's tokens
     float scale = 1.0f;
     bool any_far = false;
     // the ring is free: 64 KB of it for 32 tokens a thread
@@ -461,31 +472,33 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     if constexpr (FMT != BF_NVFP4) {
       scale = e8m0_value(row_ref[r]);
 #pragma unroll
-      for (int q = 0; q < kParts; ++q) any_far |= has_far[q][r] != 0;
+      for (int q = 0; q < kQuads; ++q) any_far |= has_far[q][r] != 0;
+      const int left = cols - first, count = left < sh.tokens / kQuads ? left : sh.tokens / kQuads;
       if (any_far)
-        far_blocks<FMT>(a, x16 + (int64_t)token0 * sh.steps * sk, (int64_t)sh.steps * sk,
-                        row0 + r < n ? row0 + r : n - 1, s0 * sk, min(s1 * sk, (int)a.kp), pt, row_ref[r],
-                        cols, far);
+        far_blocks<FMT>(a, x16 + (int64_t)(token0 + first) * sh.steps * sk, (int64_t)sh.steps * sk,
+                        row0 + r < n ? row0 + r : n - 1, s0 * sk, min(s1 * sk, (int)a.kp), row_ref[r], count,
+                        far);
       __syncwarp();
     }
-    for (int c = pt * 16; c < sh.tokens; c += 16 * kParts) {
-      uint32_t v[16];
-      tmem_ld_32x32b_x16(tmem + lanes + c, v);
+    for (int j = 0; j < sh.tokens / kQuads; j += 4) {
+      float v[4];
+      asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                   : "r"(tmem + lanes + first + j));
       tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = c + i;
+      for (int i = 0; i < 4; ++i) {
+        const int t = first + j + i;
         if (t >= cols) break;
-        const float d = __uint_as_float(v[i]);
-        float sum = FMT == BF_NVFP4 || d == 0.0f ? d : d * scale;
+        float sum = FMT == BF_NVFP4 || v[i] == 0.0f ? v[i] : v[i] * scale;
         if constexpr (FMT != BF_NVFP4) {
-          if (any_far) sum += far[(c / (16 * kParts) * 16 + i) * kDecodeWarps * 32];
+          if (any_far) sum += far[(j + i) * kDecodeWarps * 32];
         }
         if (sh.slices > 1)
           __stcg(mine + t * kRows + r, sum);
         else if (row0 + r < n)
           static_cast<T*>(a.out)[(int64_t)(token0 + t) * a.ld_out + row0 + r] =
-              from_f32<T>(a.alpha * (sum * __ldcg(xs + token0 + t)));
+              from_f32<T>(a.alpha * (sum * token_scale[t]));
       }
     }
   }
@@ -519,7 +532,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       sum.z += q.z;
       sum.w += q.w;
     }
-    const float s = __ldcg(xs + token0 + t), v[4] = {sum.x, sum.y, sum.z, sum.w};
+    const float s = token_scale[t], v[4] = {sum.x, sum.y, sum.z, sum.w};
     T* dst = static_cast<T*>(a.out) + (int64_t)(token0 + t) * a.ld_out + row0 + r;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
