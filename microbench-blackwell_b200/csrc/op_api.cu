@@ -80,8 +80,14 @@ b2g_status tensor_map(b2g_handle* h, CUtensorMap* map, CUtensorMapDataType type,
   return B2G_OK;
 }
 
-// b2g_linear: from this many tokens on the tensor-core form.
-constexpr int kTilesFrom = 9;
+// b2g_linear's form.  Nine tokens and more (the other one's limit is eight) take the tensor
+// cores' (few_tiles.cu), fewer the registers' (few_linear.cu) unless x does not fit one CTA and
+// the weights are many.  Measured (us, registers / tensor cores, 8 tokens): all of x in a CTA
+// 2048 x 2048 4.8 / 7.5, 16384 x 2048 8.2 / 9.7; beyond, 2048 x 8192 9.3 / 10.4, 8192 x 8192
+// 17.5 / 16.4, 16384 x 8192 29.2 / 22.6 (NVFP4), 8192 x 8192 22.8 / 21.8 (MXFP8).
+bool linear_tiles(const FewLinearArgs& a) {
+  return a.T > kFewTokens || (2 * a.T * a.kp > kFewXBytes && a.N * a.kp >= (int64_t)1 << 26);
+}
 
 }  // namespace
 
@@ -369,7 +375,7 @@ b2g_status b2g_linear(b2g_handle* h, const b2g_linear_desc* d, void* stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   a.err = h->d_err;
   a.wait_ns = h->wait_ns;
-  const bool tiles = d->T >= kTilesFrom;
+  const bool tiles = linear_tiles(a);
   const b2g_status st = tiles ? grow(h, few_tiles_ws_bytes(fmt, a, h->sm_count),
                                      few_tiles_counters(fmt, a, h->sm_count), s)
                               : grow(h, few_linear_ws_bytes(fmt, a, h->sm_count),

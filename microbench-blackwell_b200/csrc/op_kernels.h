@@ -76,6 +76,10 @@ cudaError_t launch_residual_norm_grad(int type, const ResidualNormGradArgs& a, i
 // Few-token product with microscaled weights (few_linear.cu).
 constexpr int kFewMaxTokens = 65536;
 constexpr int kFewMaxExtent = 1 << 24;  // N and K: indexes within a matrix's edge are 32 bits
+constexpr int kFewTokens = 8;           // at most in few_linear.cu
+// Bytes of x in a CTA there: with the warps' rings (up to 72 KB) and their sums (8 KB) two
+// CTAs fit an SM.
+constexpr int kFewXBytes = 32768;
 struct FewLinearArgs {
   int64_t T, N, K, kp;
   const void* x;

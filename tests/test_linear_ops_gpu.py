@@ -676,6 +676,17 @@ def test_products_of_infinities_and_nan(engine, fmt, T):
 
 
 @pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("T", [1, 3, 7])
+def test_few_tokens_with_many_weights(engine, fmt, T):
+    # 2^26 weights, all of x in one CTA or not
+    N, K = 4112, 16352
+    rng = np.random.default_rng(63)
+    x = rounded(rng.normal(size=(T, K)) / 64, "bf16")
+    codes, sf, w = random_weights(fmt, N, K, 64)
+    check_linear(engine, x, codes, sf, w, fmt, "bf16")
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
 @pytest.mark.parametrize("T", [5, 24])
 def test_weights_and_scales_at_odd_places(engine, fmt, T):
     # codes on 16 bytes, scales on two, neither on the allocation's start
