@@ -19,10 +19,10 @@ from ._errors import B2GError
 from ._lib import (FMT_BF16, FMT_E2M1, FMT_E2M3, FMT_E3M2, FMT_E4M3, FMT_E5M2, FMT_F16,
                    FMT_MXF4, FMT_MXF8, FMT_NVFP4, FMT_S8, FMT_TF32, FMT_U8, GemmDesc,
                    ProbeDesc)
-from ._ops import LinearOps
+from ._ops import LinearOps, block_shapes
 
 __all__ = [
-    "B2GError", "Engine", "GemmDesc", "ProbeDesc", "plan_gemm",
+    "B2GError", "Engine", "GemmDesc", "ProbeDesc", "block_shapes", "plan_gemm",
     "FMT_BF16", "FMT_E4M3", "FMT_S8", "FMT_E2M1", "FMT_MXF8", "FMT_MXF4", "FMT_NVFP4",
     "FMT_TF32", "FMT_E5M2", "FMT_E2M3", "FMT_E3M2", "FMT_F16", "FMT_U8",
 ]
