@@ -149,10 +149,14 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
 template <typename T, int HF, bool ANY>
 cudaError_t norm_launch(const ResidualNormArgs& a, int sm_count, cudaStream_t s) {
   const int64_t v = ((HF < 0 ? a.cols : a.kp) + 7) / 8;
-  // few rows: as many threads to a row as it has eights, for latency; many: four eights
-  // a thread, which keeps eight 16-byte loads in flight in each, or one warp's share of a
-  // short row
-  const int nv = v <= 32 || (a.rows < 2 * sm_count && v <= 1024) ? 1 : v <= 64 ? 2 : 4;
+  // Few rows, or a few thousand short ones: as many threads to a row as it has eights, for
+  // latency.  Many: four eights a thread, which keeps eight 16-byte loads in flight in each,
+  // or one warp's share of a short row.  Measured (bf16, us, one eight a thread / four):
+  // 1 x 8192 4.1 / 5.7, 300 x 2048 3.8 / 6.2, 4000 x 2048 18.3 / 20.4, 16384 x 2048 59.9 /
+  // 49.7, 4000 x 4096 33.4 / 30.8, 16384 x 8192 255 / 171; 20000 x 256 12.7 / 31.0.
+  const int nv = v <= 32 || (a.rows < 2 * sm_count && v <= 1024) || (v <= 256 && a.rows * v <= 1 << 20) ? 1
+                 : v <= 64 ? 2
+                           : 4;
   int64_t tpr = ((v + nv - 1) / nv + 31) / 32 * 32;
   const int rpc = tpr == 32 ? 4 : 1;
   const dim3 block((unsigned)tpr, rpc);
