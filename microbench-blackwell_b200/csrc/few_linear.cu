@@ -10,7 +10,13 @@
 // fp16: fp16 as it is, bf16 scaled per token by the power of two that brings its largest
 // value to 2^14 .. 2^15, which is exact for values down to 2^-28 of the largest (below
 // that the error is at most 2^-40 of the largest).  The second one starts along with it
-// and has its first weights on their way by the time x is laid out.
+// and has its first weights on their way by the time x is laid out.  (Every CTA laying all of
+// x out for itself, without a first kernel: 2048 x 2048 3.8 for 4.5 us, but 8192 x 8192 14.5
+// for 13.4 us.)
+//
+// Measured, one token: 8192 x 8192 NVFP4 13.4 us, MXFP4 13.4, MXFP8 18.2; 16384 x 8192 22.5,
+// 23.4, 30.4 (2.9 to 4.6 TB/s); 2048 x 2048 4.5 to 4.8 us.  About 4 us of it are the two
+// launches' latencies; beyond, instructions: 2.5 an element and lane, at 16 warps an SM.
 #include "b2g.h"
 #include "op_common.cuh"
 #include "op_kernels.h"

@@ -20,8 +20,13 @@
 namespace b2g {
 namespace {
 
-// One row per blockDim.x threads, held in registers: NV times eight elements a thread.
-// ANY: operands of any alignment.
+// One row per blockDim.x threads, held in registers: NV times eight elements a thread.  Each
+// element is read once and written once, so bytes bound it: 16384 x 8192 bf16 with norm after,
+// gate and norm before 168 us, 6.4 of the 6.5 TB/s that a copy measures; into MXFP8 codes 176 us
+// (82 %: the casts); 4095 x 5000 fp16 39 us (64 %) and one row 3.8 us: waits for memory and
+// barriers.
+// ANY: operands of any alignment, read and written as the aligned words that cover them:
+// 16384 x 8191 bf16 397 us, bound by the shifting (974 us element by element).
 template <typename T, int NV, int HF, bool ANY>
 __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormArgs a) {
   // Weights and gate are asked for before the row's sums meet, where registers allow (16-bit
