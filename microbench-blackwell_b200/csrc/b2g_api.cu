@@ -704,9 +704,8 @@ b2g_status b2g_gemm(b2g_handle* h, const b2g_gemm_desc* d, void* stream) {
     }
     uint8_t* ra = static_cast<uint8_t*>(h->sf_ws);
     uint8_t* rb = ra + na;
-    B2G_CUDA(h, launch_sf_ready((const uint8_t*)d->sfa, d->M, sf_cols, groups, 128, 128, ra,
-                                h->sm_count, s));
-    B2G_CUDA(h, launch_sf_ready((const uint8_t*)d->sfb, d->N, sf_cols, groups, bn, 256, rb,
+    B2G_CUDA(h, launch_sf_ready(sf_ready(d->sfa, d->M, sf_cols, 128, 128, ra),
+                                sf_ready(d->sfb, d->N, sf_cols, bn, 256, rb), sf_cols, groups,
                                 h->sm_count, s));
     // one ring slot: 512 x groups bytes of SFA, 1024 x groups of SFB, in kSideLine
     // lines; maps e, f (or f, g after a sparse A's metadata)

@@ -162,9 +162,17 @@ size_t meta_ready_bytes(int64_t M, int64_t K, int elem_bits = 16);
 // ring slot, per block_rows rows padded to padded_rows (NVFP4: groups 4; MXFP8: 1;
 // MXFP4: 2).
 size_t sf_ready_bytes(int64_t rows, int64_t sf_cols, int groups, int block_rows, int padded_rows);
-cudaError_t launch_sf_ready(const uint8_t* sf, int64_t rows, int64_t sf_cols, int groups,
-                            int block_rows, int padded_rows, uint8_t* ready, int sm_count,
-                            cudaStream_t s);
+struct SfReady {  // one operand's
+  const uint8_t* sf;
+  uint32_t* ready;
+  int64_t rows, blocks;
+  int block_rows, padded_shift;
+  int words;  // four scales are one aligned word
+};
+SfReady sf_ready(const void* sf, int64_t rows, int64_t sf_cols, int block_rows, int padded_rows,
+                 void* ready);
+cudaError_t launch_sf_ready(const SfReady& a, const SfReady& b, int64_t sf_cols, int groups,
+                            int sm_count, cudaStream_t s);
 // OCP MX quantisation: elem 0 = e4m3 (rows x cols bytes), 1 = e2m1 (packed rows x
 // cols/2), 2 = e5m2, 3 = e2m3, 4 = e3m2 (packed fp6); sf rows x cols/block E8M0, one
 // scale per `block` (32, the OCP MX block, or 64: the block of the 2:4-sparse

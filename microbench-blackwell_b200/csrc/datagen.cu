@@ -624,27 +624,35 @@ __global__ void meta_ready_u8_kernel(const uint32_t* canon, int64_t M, int64_t k
 // lines of 16 bytes: word (4 l + c) of each 128-row half q holds the group of
 // row 32 c + l + 128 q, the layout tcgen05.cp.32x128b.warpx4 spreads over the
 // four TMEM lane quarters.
-__global__ void sf_ready_kernel(const uint8_t* sf, int64_t rows, int64_t sf_cols, int block_rows,
-                                int padded_rows, int64_t slots, int groups, int64_t total,
-                                uint32_t* ready) {
-  for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < total;
-       idx += (int64_t)gridDim.x * blockDim.x) {
-    const int w = (int)(idx % padded_rows);
-    const int64_t t = idx / padded_rows;
-    const int kk = (int)(t % groups);
-    const int64_t bs = t / groups;
-    const int64_t slot = bs % slots, blk = bs / slots;
-    const int wl = w & 127, q = w >> 7;
-    const int local = (wl >> 2) + 32 * ((wl & 3) + 4 * q);
-    const int64_t r = blk * block_rows + local;
-    uint32_t v = 0;
-    if (local < block_rows && r < rows) {
-      const int64_t c0 = (slot * groups + kk) * 4;
+// Both operands in one launch: blockIdx.y counts A's row blocks, then B's, and a block is
+// `groups` groups of all its slots in a row, so no index is divided.
+__global__ void __launch_bounds__(256) sf_ready_kernel(const SfReady a, const SfReady b, int64_t sf_cols,
+                                                       int64_t groups) {
+  for (int64_t y = blockIdx.y; y < a.blocks + b.blocks; y += gridDim.y) {
+    const bool of_b = y >= a.blocks;
+    const int64_t blk = of_b ? y - a.blocks : y, rows = of_b ? b.rows : a.rows;
+    const int shift = of_b ? b.padded_shift : a.padded_shift, block_rows = of_b ? b.block_rows : a.block_rows;
+    const bool words = of_b ? b.words : a.words;
+    const uint8_t* sf = of_b ? b.sf : a.sf;
+    const int64_t total = groups << shift;
+    uint32_t* ready = (of_b ? b.ready : a.ready) + blk * total;
+    for (int64_t idx = blockIdx.x * 256 + threadIdx.x; idx < total; idx += gridDim.x * 256) {
+      const int w = (int)idx & ((1 << shift) - 1);
+      const int wl = w & 127, q = w >> 7;
+      const int local = (wl >> 2) + 32 * ((wl & 3) + 4 * q);
+      const int64_t r = blk * block_rows + local, c0 = (idx >> shift) * 4;
+      uint32_t v = 0;
+      if (local < block_rows && r < rows) {
+        if (words && c0 < sf_cols) {
+          v = *reinterpret_cast<const uint32_t*>(sf + r * sf_cols + c0);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c0 + j < sf_cols) v |= (uint32_t)sf[r * sf_cols + c0 + j] << (8 * j);
+          for (int j = 0; j < 4; ++j)
+            if (c0 + j < sf_cols) v |= (uint32_t)sf[r * sf_cols + c0 + j] << (8 * j);
+        }
+      }
+      ready[idx] = v;
     }
-    ready[idx] = v;
   }
 }
 
@@ -722,15 +730,27 @@ size_t sf_ready_bytes(int64_t rows, int64_t sf_cols, int groups, int block_rows,
          (size_t)padded_rows * 4;
 }
 
-cudaError_t launch_sf_ready(const uint8_t* sf, int64_t rows, int64_t sf_cols, int groups,
-                            int block_rows, int padded_rows, uint8_t* ready, int sm_count,
-                            cudaStream_t s) {
-  const int64_t slots = (sf_cols + 4 * groups - 1) / (4 * groups);
-  const int64_t blocks = (rows + block_rows - 1) / block_rows;
-  const int64_t total = blocks * slots * groups * padded_rows;  // words: sf_ready_bytes(...) / 4
-  sf_ready_kernel<<<grid_for(total, sm_count), 256, 0, s>>>(sf, rows, sf_cols, block_rows,
-                                                            padded_rows, slots, groups, total,
-                                                            reinterpret_cast<uint32_t*>(ready));
+SfReady sf_ready(const void* sf, int64_t rows, int64_t sf_cols, int block_rows, int padded_rows,
+                 void* ready) {
+  SfReady r;
+  r.sf = static_cast<const uint8_t*>(sf);
+  r.rows = rows;
+  r.blocks = (rows + block_rows - 1) / block_rows;
+  r.ready = static_cast<uint32_t*>(ready);
+  r.block_rows = block_rows;
+  r.padded_shift = padded_rows == 128 ? 7 : 8;
+  r.words = sf_cols % 4 == 0 && (reinterpret_cast<uintptr_t>(sf) & 3) == 0;
+  return r;
+}
+
+cudaError_t launch_sf_ready(const SfReady& a, const SfReady& b, int64_t sf_cols, int groups,
+                            int sm_count, cudaStream_t s) {
+  const int64_t all = (sf_cols + 4 * groups - 1) / (4 * groups) * groups;  // of a row block
+  const int64_t blocks = a.blocks + b.blocks;
+  int64_t gx = all, most = (int64_t)sm_count * 16 / blocks;  // 256 words a CTA and turn
+  gx = gx < most ? gx : most;
+  const dim3 grid((unsigned)(gx < 1 ? 1 : gx), (unsigned)(blocks < 65535 ? blocks : 65535));
+  sf_ready_kernel<<<grid, 256, 0, s>>>(a, b, sf_cols, all);
   return cudaGetLastError();
 }
 
