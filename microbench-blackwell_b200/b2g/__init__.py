@@ -19,7 +19,7 @@ from ._errors import B2GError
 from ._lib import (FMT_BF16, FMT_E2M1, FMT_E2M3, FMT_E3M2, FMT_E4M3, FMT_E5M2, FMT_F16,
                    FMT_MXF4, FMT_MXF8, FMT_NVFP4, FMT_S8, FMT_TF32, FMT_U8, GemmDesc,
                    ProbeDesc)
-from ._ops import LinearOps, block_shapes
+from ._ops import LinearOps, _Torch, block_shapes
 
 __all__ = [
     "B2GError", "Engine", "GemmDesc", "ProbeDesc", "block_shapes", "plan_gemm",
@@ -27,6 +27,8 @@ __all__ = [
     "FMT_TF32", "FMT_E5M2", "FMT_E2M3", "FMT_E3M2", "FMT_F16", "FMT_U8",
 ]
 
+
+torch = _Torch(globals())
 
 # bits per element of the packed formats whose tensors hold bytes
 _PACKED_BITS = {FMT_E2M1: 4, FMT_E2M3: 6, FMT_E3M2: 6, FMT_MXF4: 4, FMT_NVFP4: 4}
@@ -37,11 +39,27 @@ def _ptr(t) -> int:
 
 
 def _stream(stream) -> int:
-    import torch
-
     if stream is None:
-        stream = torch.cuda.current_stream()
+        # the current stream of the current device, without an object for it
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return int(stream.cuda_stream)
+
+
+def _gemm_desc(A, B, C_out, fmt, M, N, K, alpha, cta_group, tile_n, stages, max_ctas, ab_mode,
+               sparse, meta, sfa, sfb, lda, ldb, ldc, meta_layout, raster_m, m_sub, split_tail,
+               b_format, mx_scale, instruction):
+    # stored elements per 8 bits of a row (1 for the byte and wider formats,
+    # whose tensors hold whole elements)
+    bits, b_bits = _PACKED_BITS.get(fmt, 8), _PACKED_BITS.get(b_format or fmt, 8)
+    if K is None:
+        K = A.shape[1] * 8 // bits * (2 if sparse else 1)
+    return GemmDesc(
+        fmt, sparse, M if M is not None else A.shape[0], N if N is not None else B.shape[0], K,
+        lda if lda is not None else A.stride(0) * 8 // bits,
+        ldb if ldb is not None else B.stride(0) * 8 // b_bits,
+        ldc if ldc is not None else C_out.stride(0), _ptr(A), _ptr(B), _ptr(C_out), _ptr(sfa),
+        _ptr(sfb), _ptr(meta), alpha, cta_group, ab_mode, tile_n, stages, max_ctas, meta_layout,
+        raster_m, m_sub, split_tail, b_format, mx_scale, instruction)
 
 
 class Engine(LinearOps):
@@ -91,13 +109,12 @@ class Engine(LinearOps):
         sfb) to those element types (kind::mxf8f6f4); instruction = 1 issues the
         weight-stationary tcgen05.mma.ws (.ws.sp when sparse).
         """
-        d = self._desc(A, B, C_out, fmt, M=M, N=N, K=K, alpha=alpha, cta_group=cta_group,
-                       tile_n=tile_n, stages=stages, max_ctas=max_ctas, ab_mode=ab_mode,
-                       sparse=sparse, meta=meta, sfa=sfa, sfb=sfb, lda=lda, ldb=ldb, ldc=ldc,
-                       meta_layout=meta_layout, raster_m=raster_m, m_sub=m_sub,
-                       split_tail=split_tail, b_format=b_format, mx_scale=mx_scale,
-                       instruction=instruction)
-        self._ok(self.lib.b2g_gemm(self.h, C.byref(d), _stream(stream)), "b2g_gemm")
+        d = _gemm_desc(A, B, C_out, fmt, M, N, K, alpha, cta_group, tile_n, stages, max_ctas, ab_mode,
+                       sparse, meta, sfa, sfb, lda, ldb, ldc, meta_layout, raster_m, m_sub,
+                       split_tail, b_format, mx_scale, instruction)
+        st = self.lib.b2g_gemm(self.h, C.byref(d), _stream(stream))
+        if st:
+            self._ok(st, "b2g_gemm")
         return C_out
 
     @staticmethod
@@ -105,18 +122,9 @@ class Engine(LinearOps):
               stages=0, max_ctas=0, ab_mode=0, sparse=0, meta=None, sfa=None, sfb=None,
               lda=None, ldb=None, ldc=None, meta_layout=0, raster_m=0, m_sub=0,
               split_tail=0, b_format=0, mx_scale=0, instruction=0):
-        # stored elements per 8 bits of a row (1 for the byte and wider formats,
-        # whose tensors hold whole elements)
-        bits, b_bits = _PACKED_BITS.get(fmt, 8), _PACKED_BITS.get(b_format or fmt, 8)
-        if K is None:
-            K = A.shape[1] * 8 // bits * (2 if sparse else 1)
-        return GemmDesc(
-            fmt, sparse, M if M is not None else A.shape[0], N if N is not None else B.shape[0], K,
-            lda if lda is not None else A.stride(0) * 8 // bits,
-            ldb if ldb is not None else B.stride(0) * 8 // b_bits,
-            ldc if ldc is not None else C_out.stride(0), _ptr(A), _ptr(B), _ptr(C_out), _ptr(sfa),
-            _ptr(sfb), _ptr(meta), alpha, cta_group, ab_mode, tile_n, stages, max_ctas, meta_layout,
-            raster_m, m_sub, split_tail, b_format, mx_scale, instruction)
+        return _gemm_desc(A, B, C_out, fmt, M, N, K, alpha, cta_group, tile_n, stages, max_ctas,
+                          ab_mode, sparse, meta, sfa, sfb, lda, ldb, ldc, meta_layout, raster_m, m_sub,
+                          split_tail, b_format, mx_scale, instruction)
 
     def gemm_host(self, A, B, C_out, fmt: int, *, alpha: float = 1.0, stream=None, **kw):
         """b2g_gemm_host: A, B, C_out are HOST tensors (pin them for full copy speed);

@@ -13,16 +13,19 @@ from ._errors import B2GError
 
 
 class _Torch:
-    """torch, imported at its first use: the package itself loads without it."""
+    """torch in a module's names, imported at its first use: the package loads without it."""
+
+    def __init__(self, names):
+        self._names = names
 
     def __getattr__(self, name):
         import torch as module
 
-        globals()["torch"] = module
+        self._names["torch"] = module
         return getattr(module, name)
 
 
-torch = _Torch()
+torch = _Torch(globals())
 _TYPES = {}  # b2g_dtype of a torch dtype
 _BLOCK = {_lib.FMT_NVFP4: 16, _lib.FMT_MXF4: 32, _lib.FMT_MXF8: 32}
 
