@@ -7,13 +7,14 @@
 // by a first kernel, is operand B, up to 128 tokens of it; sums stay in tensor memory until
 // the end.  A decoded weight then serves all tokens for one instruction's issue.
 //
-// Measured, 16384 x 8192, 16 tokens: NVFP4 21.9 us, MXFP4 23.6, MXFP8 34.2; 64 tokens 25.9,
-// 28.8, 37.9; 128 tokens 43.7, 46.8, 47.2 (x is read from L2 by every
-// CTA, 64 KB for each 16 KB of codes); 2048 x 2048, 16 tokens 8 to 9 us.  Of the 23.6 us about 6 pass
+// Measured, 16384 x 8192, 16 tokens: NVFP4 21.4 us, MXFP4 23.3, MXFP8 34.3; 64 tokens 25.7,
+// 28.5, 37.9; 128 tokens 43.6, 46.4, 47.3 (x is read from L2 by every CTA, 64 KB for each
+// 16 KB of codes); 2048 x 2048, 16 tokens 8 to 9 us.  Of MXFP4's 16 tokens about 6 us pass
 // before the first step is decoded (x's layout, launch, first copies) and 2 after the last;
-// between, a step of 256 elements x 128 rows takes 0.43 us, the issue of its 16 MMAs at about
-// 50 cycles each: 4.9 TB/s of weights.  MXFP8's steps have half as many products for their
-// bytes and run at 6 TB/s.
+// between, a step of 256 elements x 128 rows takes 0.43 us, 4.9 TB/s of weights, MXFP8's, of half
+// as many elements, 6 TB/s.  Tensor pipe (11 % busy), issue slots (53 %) and memory (70 % in the
+// loop) are none of them full: it is the chain copy, decoding, products, and neither more
+// buffers nor more ring slots shortened it.
 #include <cuda.h>
 
 #include "b2g.h"
@@ -194,8 +195,12 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   __shared__ uint8_t has_far[kQuads][kRows];
   constexpr int sk = step_k(FMT);
   constexpr uint32_t a_cols = sk / 2;               // TMEM columns of a decoded step
-  constexpr int buffers = FMT == BF_MXF8 ? 4 : 3;   // of them
-  static_assert(buffers <= kMaxBuffers && 128 + buffers * a_cols <= 512, "tensor memory");
+  // Of them, and of ring slots, an even number: each is then always filled or read by the same
+  // group, which has waited for every one of its barriers' phases and cannot take one for the
+  // next but one.
+  constexpr int buffers = FMT == BF_MXF8 ? 4 : 2;
+  static_assert(buffers % kGroups == 0 && buffers <= kMaxBuffers && 128 + buffers * a_cols <= 512,
+                "buffers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = (int)blockIdx.x / sh.slices, slice = (int)blockIdx.x % sh.slices;
   const int s0 = (int)((unsigned)sh.steps * (unsigned)slice / (unsigned)sh.slices);
@@ -559,7 +564,7 @@ TileShape tile_shape(int fmt, const FewLinearArgs& a, int sm_count) {
   n = n < s.steps / 2 ? n : s.steps / 2;
   s.slices = n < 1 ? 1 : n;
   const int slot = kRows * kCodeBytes + s.tokens * step_k(fmt) * 2 + kScaleBytes;
-  s.stages = (220 * 1024) / slot < kMaxStages ? (220 * 1024) / slot : kMaxStages;
+  s.stages = (220 * 1024) / slot < kMaxStages ? (220 * 1024) / slot / kGroups * kGroups : kMaxStages;
   s.smem = s.stages * slot + 1024;
   // tensor memory is taken whole: one CTA an SM
   if (s.smem < 120 * 1024) s.smem = 120 * 1024;
