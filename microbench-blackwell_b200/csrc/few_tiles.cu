@@ -291,10 +291,10 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         round ^= 1u;
       }
     }
-    // every copy lands before the CTA ends
+    // every copy lands before the CTA ends, however short the caller's limit is
     int none = 0;
     for (int i = asked > sh.stages ? asked - sh.stages : 0; i < asked; ++i)
-      mbar_wait(full(i % sh.stages), (uint32_t)(i / sh.stages) & 1u, &none, nullptr, 0, a.wait_ns);
+      mbar_wait(full(i % sh.stages), (uint32_t)(i / sh.stages) & 1u, &none, nullptr, 0, 0);
     __syncwarp();
   } else if (warp == kDecodeWarps) {
     // ---- products
@@ -327,7 +327,7 @@ few_tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     tc_commit<1>(done, on);
     // nothing of this warp is in flight when tensor memory is given back
     int none = 0;
-    if (!mbar_wait(done, 0, &none, nullptr, 0, a.wait_ns) && on) {
+    if (!mbar_wait(done, 0, &none, nullptr, 0, 0) && on) {
       aborted = 1;
       if (a.err) atomicOr(a.err, ERRW_TIMEOUT_MMA);
     }

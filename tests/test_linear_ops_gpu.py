@@ -724,6 +724,32 @@ def test_tens_of_tokens_repeat_to_the_bit_on_another_stream_and_in_a_graph(engin
     engine.check()
 
 
+def test_tens_of_tokens_with_the_shortest_wait_limit(engine):
+    # under a limit of a microsecond a call either is right or reports that a wait ran out; nothing
+    # is left behind, and the next call with the usual limit is right
+    codes, sf, _ = random_weights("nvfp4", 1000, 8192, 65)
+    c, s = torch.from_numpy(codes).cuda(), torch.from_numpy(sf).cuda()
+    x = dev(np.random.default_rng(66).normal(size=(20, 8192)) / 64, torch.bfloat16)
+    first, out = (torch.empty(20, 1000, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    engine.linear(x, c, s, first, FMT["nvfp4"])
+    engine.check()
+    for _ in range(20):
+        engine.set_wait_limit(1000)
+        try:
+            out.zero_()
+            engine.linear(x, c, s, out, FMT["nvfp4"])
+            engine.check()
+            assert torch.equal(first, out)
+        except b2g.B2GError as e:
+            assert e.status == b2g._lib.B2G_ERR_TIMEOUT
+        finally:
+            engine.set_wait_limit(0)
+        out.zero_()
+        engine.linear(x, c, s, out, FMT["nvfp4"])
+        engine.check()
+        assert torch.equal(first, out)
+
+
 @pytest.mark.parametrize("typ", list(TYPE))
 @pytest.mark.parametrize("cols", [1, 2, 7, 9, 15, 17, 31, 257])
 def test_norm_passes_of_narrow_rows_at_odd_places(engine, typ, cols):
