@@ -1,6 +1,6 @@
 // few_linear.cu -- y = alpha * x . W^T of one to eight tokens (16-bit x) with microscaled
 // weights, for decoding: every weight is read once and used a handful of times, so the
-// kernel is bound by the weights' bytes.
+// weights' bytes are the floor.
 //
 // Codes become fp16 pairs in registers and go into mma.sync m16n8k16 with the weights
 // as the 16-row operand and the tokens as the 8 columns: tcgen05 takes its operands
@@ -16,7 +16,7 @@
 //
 // Measured, one token: 8192 x 8192 NVFP4 13.4 us, MXFP4 13.4, MXFP8 18.2; 16384 x 8192 22.5,
 // 23.4, 30.4 (2.9 to 4.6 TB/s); 2048 x 2048 4.5 to 4.8 us.  About 4 us of it are the two
-// launches' latencies; beyond, instructions: 2.5 an element and lane, at 16 warps an SM.
+// launches' latencies; beyond, instructions: 2.4 an element and lane, at 16 warps an SM.
 #include "b2g.h"
 #include "op_common.cuh"
 #include "op_kernels.h"
