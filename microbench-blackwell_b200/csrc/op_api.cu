@@ -135,7 +135,8 @@ b2g_status b2g_block_quantize(b2g_handle* h, const b2g_block_quant_desc* d, void
   a.rand_vec = d->rand && rows_aligned(d->rand, d->ld_rand, 1, 8);
   uint32_t bits;
   memcpy(&bits, &d->scale, 4);
-  const bool pow2 = (bits & 0x7FFFFFu) == 0 && (bits >> 23) != 0;
+  // a power of two that an NVFP4 scale's reciprocal, at most 2^9, can take in and stay finite
+  const bool pow2 = (bits & 0x7FFFFFu) == 0 && (bits >> 23) != 0 && d->scale <= 0x1p100f;
   DeviceGuard g(h->device);
   B2G_CUDA(h, launch_block_quant(fmt, d->in_type, pow2, a, reinterpret_cast<cudaStream_t>(stream)));
   return B2G_OK;

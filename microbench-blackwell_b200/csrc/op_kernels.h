@@ -23,7 +23,7 @@ struct BlockQuantArgs {
   int in_vec;    // every row of `in` starts on 16 bytes
   int rand_vec;  // every row of `rand` starts on 8 bytes
 };
-// fmt: BlockFmt; type: b2g_dtype; pow2: scale is a power of two
+// fmt: BlockFmt; type: b2g_dtype; pow2: scale is a power of two, 2^100 at most
 cudaError_t launch_block_quant(int fmt, int type, bool pow2, const BlockQuantArgs& a,
                                cudaStream_t s);
 

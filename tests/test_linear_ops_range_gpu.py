@@ -1,0 +1,51 @@
+"""Operators around a linear layer at the ends of their range: blocks of zeros, tiny and huge
+blocks under a scale, bytes next to the point where a code goes up, rows of any magnitude."""
+import numpy as np
+import pytest
+import torch
+
+import linear_ops_ref as ref
+from test_linear_ops_gpu import FMT, TYPE, check_cast, code_buffers, dev, rounded
+
+pytestmark = pytest.mark.gpu
+
+
+def cast_and_check(engine, fmt, typ, x, scale, rand=None):
+    """Both ways against the definition, and the read-back finite; x * scale is exact."""
+    rows, cols = x.shape
+    (c, s), (ct, st) = code_buffers(fmt, rows, cols), code_buffers(fmt, cols, rows)
+    r = None if rand is None else dev(rand, torch.uint8, fill=0)
+    engine.quantize_block(FMT[fmt], dev(x, TYPE[typ]), c, s, codes_t=ct, sf_t=st, scale=scale, rand=r)
+    check_cast(c, s, x * scale, fmt, rand)
+    check_cast(ct, st, x.T * scale, fmt, None if rand is None else rand.T)
+    c1, s1 = code_buffers(fmt, rows, cols)
+    engine.quantize_block(FMT[fmt], dev(x, TYPE[typ]), c1, s1, scale=scale, rand=r)
+    assert torch.equal(c, c1) and torch.equal(s, s1)
+    out = torch.empty(rows, cols, dtype=torch.float32, device="cuda")
+    engine.dequantize_block(FMT[fmt], c, s, out)
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("stochastic", [False, True])
+@pytest.mark.parametrize("scale", [2.0, 64.0, 4096.0])
+@pytest.mark.parametrize("typ", list(TYPE))
+@pytest.mark.parametrize("fmt", list(FMT))
+def test_cast_of_zero_and_tiny_blocks_with_a_scale(engine, fmt, typ, scale, stochastic):
+    rng = np.random.default_rng(70)
+    x = rng.normal(size=(70, 130))
+    x[3], x[4] = 0.0, -0.0          # masked tokens
+    x[:, 7] = 0.0                   # a feature no token uses
+    x[10:42, 32:64] = 0.0           # a zero block both ways
+    x[43:, :32] *= 2.0 ** -124      # bf16, fp32: next to the least of the type; fp16: zeros
+    x[50, 64:96] = 2.0 ** -126 * (np.arange(32) % 5 - 2)
+    x[51, 64:] = 2.0 ** -24 * (np.arange(66) % 3 - 1)
+    rand = rng.integers(0, 256, x.shape) if stochastic else None
+    cast_and_check(engine, fmt, typ, rounded(x, typ), scale, rand)
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", list(FMT))
+def test_cast_with_a_scale_near_the_largest(engine, fmt, typ):
+    x = np.random.default_rng(73).normal(size=(40, 96)) * 2.0 ** -115
+    x[5], x[:, 9], x[7, 32:64] = 0.0, 0.0, 2.0 ** -126
+    cast_and_check(engine, fmt, typ, rounded(x, typ), 2.0 ** 120)
