@@ -443,6 +443,8 @@ __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s, 
   uint32_t bits;
   if constexpr (QM == Q_DIVIDE)
     bits = __float_as_uint(s.inv != 0.0f ? fabsf(x / s.value) * down : 0.0f);
+  else if constexpr (QM == Q_EXACT)
+    bits = __float_as_uint(__fmul_ru(fabsf(x), down));  // x is the quotient already
   else
     bits = __float_as_uint(__fmul_ru(fabsf(x), mult));
   // 256 r + 128: the byte above a half, one permutation
@@ -468,9 +470,11 @@ __device__ __forceinline__ void encode8(const float2 (&in)[4], const BlockScale&
     mult = s.inv;
   }
   if constexpr (SR) {
-    const float m = mult * (FMT == BF_MXF8 ? 0x1p-120f : 0x1p-126f);
+    // MX: 1 / s and the format's shift are two products, as one may leave fp32's range
+    const float m = mult * 0x1p-126f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (QM == Q_EXACT) x[i] = mul2(x[i], both(mult));
       const uint32_t word = i < 2 ? rnd.x : rnd.y;
       q[i].x = round_stochastic<FMT, QM>(x[i].x, s, m, word, 2 * (i & 1));
       q[i].y = round_stochastic<FMT, QM>(x[i].y, s, m, word, 2 * (i & 1) + 1);

@@ -49,3 +49,14 @@ def test_cast_with_a_scale_near_the_largest(engine, fmt, typ):
     x = np.random.default_rng(73).normal(size=(40, 96)) * 2.0 ** -115
     x[5], x[:, 9], x[7, 32:64] = 0.0, 0.0, 2.0 ** -126
     cast_and_check(engine, fmt, typ, rounded(x, typ), 2.0 ** 120)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -30, 2.0 ** 12])
+@pytest.mark.parametrize("typ", list(TYPE))
+@pytest.mark.parametrize("fmt", ["mxf4", "mxf8"])
+def test_stochastic_cast_of_large_blocks(engine, fmt, typ, scale):
+    rng = np.random.default_rng(71)
+    # a row's magnitude, up to what the type and the product with scale hold
+    top = 15 if typ == "f16" else 110
+    x = np.clip(rng.normal(size=(48, 96)), -3, 3) * 2.0 ** np.linspace(-10, top - 3, 48)[:, None]
+    cast_and_check(engine, fmt, typ, rounded(x, typ), scale, rng.integers(0, 256, x.shape))
