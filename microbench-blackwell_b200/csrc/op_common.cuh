@@ -431,11 +431,12 @@ __device__ __forceinline__ BlockScale block_scale(float amax) {
 // when its fraction and (r + 1/2) / 256 together reach the next step.  |x / s| is scaled so
 // that the format's lowest binade becomes the lowest normal one of fp32: the bits of the
 // result then are the magnitude code with the fraction below it, subnormal codes included,
-// and (r + 1/2) / 256 of a step is added to them as an integer.  Q_SNAP: a fraction that
-// with r reaches the step exactly must not come out below; 1 / s and the product are
-// rounded up, and no other quotient lies that near (the thresholds have 12 bits).
+// and (r + 1/2) / 256 of a step is added to them as an integer.  x: the quotient already
+// (Q_DIVIDE: the element).  Q_SNAP: a fraction that with r reaches the step exactly must not
+// come out below; 1 / s is rounded up, and the product then does not fall below a threshold
+// that x / s reaches.  No other quotient lies that near: the thresholds have 12 bits.
 template <int FMT, int QM>
-__device__ __forceinline__ float round_stochastic(float x, const BlockScale& s, float mult,
+__device__ __forceinline__ float round_stochastic(float x, const BlockScale& s,
                                                   uint32_t word, int byte) {
   constexpr float down = FMT == BF_MXF8 ? 0x1p-120f : 0x1p-126f;
   constexpr float up = FMT == BF_MXF8 ? 0x1p120f : 0x1p126f;
@@ -443,10 +444,8 @@ __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s, 
   uint32_t bits;
   if constexpr (QM == Q_DIVIDE)
     bits = __float_as_uint(s.inv != 0.0f ? fabsf(x / s.value) * down : 0.0f);
-  else if constexpr (QM == Q_EXACT)
-    bits = __float_as_uint(__fmul_ru(fabsf(x), down));  // x is the quotient already
   else
-    bits = __float_as_uint(__fmul_ru(fabsf(x), mult));
+    bits = __float_as_uint(__fmul_ru(fabsf(x), down));  // x is the quotient already
   // 256 r + 128: the byte above a half, one permutation
   const uint32_t r = __byte_perm(word, 0x80u, 0x5504u | (uint32_t)(byte << 4));
   bits = (r * (1u << (frac - 16)) + bits) & (0xFFFFFFFFu << frac);
@@ -470,14 +469,14 @@ __device__ __forceinline__ void encode8(const float2 (&in)[4], const BlockScale&
     mult = s.inv;
   }
   if constexpr (SR) {
-    // MX: 1 / s and the format's shift are two products, as one may leave fp32's range
-    const float m = mult * 0x1p-126f;
+    // 1 / s and the format's shift are two products: as one it may leave fp32's range (MX), or
+    // be subnormal and lose bits (NVFP4)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (QM == Q_EXACT) x[i] = mul2(x[i], both(mult));
+      if (QM != Q_DIVIDE) x[i] = mul2(x[i], both(mult));
       const uint32_t word = i < 2 ? rnd.x : rnd.y;
-      q[i].x = round_stochastic<FMT, QM>(x[i].x, s, m, word, 2 * (i & 1));
-      q[i].y = round_stochastic<FMT, QM>(x[i].y, s, m, word, 2 * (i & 1) + 1);
+      q[i].x = round_stochastic<FMT, QM>(x[i].x, s, word, 2 * (i & 1));
+      q[i].y = round_stochastic<FMT, QM>(x[i].y, s, word, 2 * (i & 1) + 1);
     }
   } else {
 #pragma unroll

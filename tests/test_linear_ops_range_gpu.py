@@ -60,3 +60,44 @@ def test_stochastic_cast_of_large_blocks(engine, fmt, typ, scale):
     top = 15 if typ == "f16" else 110
     x = np.clip(rng.normal(size=(48, 96)), -3, 3) * 2.0 ** np.linspace(-10, top - 3, 48)[:, None]
     cast_and_check(engine, fmt, typ, rounded(x, typ), scale, rng.integers(0, 256, x.shape))
+
+
+def around_the_step(fmt, s, q):
+    """The byte from which |x| = q * s goes up, and the one before (clipped to a byte)."""
+    grid = ref.GRID[fmt]
+    lo = np.clip(np.searchsorted(grid, q, side="right") - 1, 0, len(grid) - 2)
+    f = (q - grid[lo]) / (grid[lo + 1] - grid[lo])
+    r = np.ceil(256 * (1 - f) - 0.5)
+    return np.clip(np.stack([r - 1, r]), 0, 255).astype(np.int64)
+
+
+def blocks_of(first, elements, fmt):
+    """Rows of one block: `first`, which fixes the scale, then the elements."""
+    n = ref.BLOCK[fmt] - 1
+    e = np.resize(elements, -(-len(elements) // n) * n).reshape(-1, n)
+    return np.concatenate([np.broadcast_to(first, (len(e), 1)), e], 1)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -8, 256.0])
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+def test_stochastic_nvfp4_of_every_value_at_its_step(engine, typ, scale):
+    # every 16-bit magnitude whose code is neither 0 for all bytes nor saturated, over every
+    # ue4m3 scale, with the two bytes between which its code changes
+    bits = np.arange(1, 1 << 15, dtype=np.int32)
+    v = torch.from_numpy(bits.astype(np.int16)).view(TYPE[typ]).double().numpy()
+    v = v[np.isfinite(v)]
+    xs, rs = [], []
+    for s in ref.E4M3[1:]:
+        first = 6 * s / scale
+        if rounded(np.array([first]), typ)[0] != first:
+            continue  # beyond fp16
+        el = v[(v >= 2.0 ** -10 * s / scale) & (v <= first)]
+        el = np.concatenate([el, -el[::3]])
+        x = blocks_of(first, el, "nvfp4")
+        for r in around_the_step("nvfp4", s, np.abs(x) * scale / s):
+            xs.append(x), rs.append(r)
+    x, r = np.concatenate(xs), np.concatenate(rs)
+    x, r = np.pad(x, ((0, 0), (0, 16))), np.pad(r, ((0, 0), (0, 16)))  # whole 32 columns
+    c, sf = code_buffers("nvfp4", *x.shape)
+    engine.quantize_block(FMT["nvfp4"], dev(x, TYPE[typ]), c, sf, scale=scale, rand=dev(r, torch.uint8, fill=0))
+    check_cast(c, sf, x * scale, "nvfp4", r)
