@@ -435,6 +435,8 @@ __device__ __forceinline__ BlockScale block_scale(float amax) {
 // (Q_DIVIDE: the element).  Q_SNAP: a fraction that with r reaches the step exactly must not
 // come out below; 1 / s is rounded up, and the product then does not fall below a threshold
 // that x / s reaches.  No other quotient lies that near: the thresholds have 12 bits.
+// The shift rounds towards zero: what it drops below a subnormal code's 22 (20) bits of
+// fraction must not lift an fp32 quotient to a threshold that it lies under.
 template <int FMT, int QM>
 __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s,
                                                   uint32_t word, int byte) {
@@ -443,9 +445,9 @@ __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s,
   constexpr int frac = FMT == BF_MXF8 ? 20 : 22;  // bits below the code
   uint32_t bits;
   if constexpr (QM == Q_DIVIDE)
-    bits = __float_as_uint(s.inv != 0.0f ? fabsf(x / s.value) * down : 0.0f);
+    bits = __float_as_uint(s.inv != 0.0f ? __fmul_rz(fabsf(x / s.value), down) : 0.0f);
   else
-    bits = __float_as_uint(__fmul_ru(fabsf(x), down));  // x is the quotient already
+    bits = __float_as_uint(__fmul_rz(fabsf(x), down));  // x is the quotient already
   // 256 r + 128: the byte above a half, one permutation
   const uint32_t r = __byte_perm(word, 0x80u, 0x5504u | (uint32_t)(byte << 4));
   bits = (r * (1u << (frac - 16)) + bits) & (0xFFFFFFFFu << frac);

@@ -101,3 +101,24 @@ def test_stochastic_nvfp4_of_every_value_at_its_step(engine, typ, scale):
     c, sf = code_buffers("nvfp4", *x.shape)
     engine.quantize_block(FMT["nvfp4"], dev(x, TYPE[typ]), c, sf, scale=scale, rand=dev(r, torch.uint8, fill=0))
     check_cast(c, sf, x * scale, "nvfp4", r)
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+def test_stochastic_cast_of_fp32_next_to_each_step(engine, fmt):
+    # x = s (n + 1 - (r + 1/2) / 256) steps goes up, its fp32 neighbour below does not
+    grid = ref.GRID[fmt]
+    xs, rs = [], []
+    for s in (ref.E4M3[[1, 9, 60, 77, 101, 126]] if fmt == "nvfp4" else 2.0 ** np.array([-100, -3, 0, 20, 90])):
+        lo, r = np.meshgrid(np.arange(len(grid) - 1), np.arange(0, 256, 5 if fmt == "mxf8" else 1))
+        lo, r = lo.ravel(), r.ravel()
+        at = (s * (grid[lo] + (grid[lo + 1] - grid[lo]) * (1 - (r + 0.5) / 256))).astype(np.float32)
+        for x in (at, np.nextafter(at, np.float32(0))):
+            e = blocks_of(s * grid[-1], x.astype(np.float64), fmt)
+            xs.append(e)
+            rs.append(np.concatenate([np.zeros((len(e), 1)), np.resize(r, (len(e), e.shape[1] - 1))], 1))
+    x, r = np.concatenate(xs), np.concatenate(rs).astype(np.int64)
+    if fmt == "nvfp4":
+        x, r = np.pad(x, ((0, 0), (0, 16))), np.pad(r, ((0, 0), (0, 16)))
+    c, sf = code_buffers(fmt, *x.shape)
+    engine.quantize_block(FMT[fmt], dev(x, torch.float32), c, sf, rand=dev(r, torch.uint8, fill=0))
+    check_cast(c, sf, x, fmt, r)
