@@ -17,9 +17,10 @@ namespace {
 // With v^ = v r2, y^ = y r1, p = w_pre dh, q = beta w_post g:
 //   dv = dx_out + r2 (p - v^ mean(p v^)),  dx = alpha dv,  dw_pre = sum dh v^
 //   dy = r1 (q dv - y^ mean(q dv y^)),  dgate = beta sum z dv,  dw_post = sum beta g dv y^
-// mean(q dv y^) follows from sums that need no dv: with A = sum p v, B = sum q y
-// (dx_out + r2 p), C = sum q y v it is r1 (B - r2^3 A C / D) / D.  So one reduction per
-// row gives both means.
+// mean(q dv y^) follows from sums that need no dv: with A = sum p v^, B = sum q y^
+// (dx_out + r2 p), C = sum q y^ v^ it is (B - r2 (A / D) C) / D.  So one reduction per
+// row gives both means.  Every product is taken with v^ and y^, never with a power of r2 or
+// r1 by itself: a row's gradients then have the range of the formula, whatever its size.
 
 // Rows of up to 8192 columns go through grad_rows_kernel in one pass; wider ones, which do not
 // fit a CTA's registers and shared memory, through a pass for the means and one down the
@@ -325,7 +326,8 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
         unpack4x2(kKeep ? wq[j] : get(a.w_pre, 0, 1, j), w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          dwq[j][i] = fma2(p[i], mul2(v[i], both(r2)), dwq[j][i]);
+          v[i] = mul2(v[i], both(r2));
+          dwq[j][i] = fma2(p[i], v[i], dwq[j][i]);
           p[i] = mul2(p[i], w[i]);
           sum[0] = fma2(p[i], v[i], sum[0]);
           u[j][i] = fma2(p[i], both(r2), u[j][i]);
@@ -336,7 +338,7 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
         fetch(slot, 3, j, y);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 qy = mul2(gw[j][i], y[i]);
+          const float2 qy = mul2(gw[j][i], mul2(y[i], both(rp)));
           sum[1] = fma2(qy, u[j][i], sum[1]);
           sum[2] = fma2(qy, v[i], sum[2]);
         }
@@ -352,8 +354,9 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
     } else if (has_h || norm_y) {
       row_sum(s, red[(r - r0) & 1]);
     }
-    const float c2 = r2 * r2 * r2 * s[0] * mean;
-    const float c1 = a.beta * (rp * rp * rp) * (s[1] - c2 * s[2]) * mean;
+    // of v^ and of y^
+    const float c2 = r2 * (s[0] * mean);
+    const float c1 = rp * ((s[1] - c2 * s[2]) * mean * a.beta), rb = rp * a.beta;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!on[j]) continue;
@@ -363,7 +366,7 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
         float2 v[4];
         fetch(slot, 1, j, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dv[i] = fma2(v[i], both(-c2), dv[i]);
+        for (int i = 0; i < 4; ++i) dv[i] = fma2(mul2(v[i], both(r2)), both(-c2), dv[i]);
       }
       if (out_x) {
 #pragma unroll
@@ -373,12 +376,12 @@ grad_rows_kernel(const ResidualNormGradArgs a, const GradRows plan, float* part,
       if (has_y) {
         float2 y[4];
         fetch(slot, 3, j, y);
-        // dy = beta r1 g w dv - y c1
+        // dy = beta r1 g w dv - y^ c1
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 d = mul2(dv[i], both(rp));
-          z[j][i] = fma2(y[i], d, z[j][i]);
-          o[i] = mul2(gw[j][i], mul2(d, both(a.beta)));
+          y[i] = mul2(y[i], both(rp));
+          z[j][i] = fma2(y[i], dv[i], z[j][i]);
+          o[i] = mul2(gw[j][i], mul2(dv[i], both(rb)));
           if (norm_y) o[i] = fma2(y[i], both(-c1), o[i]);
         }
         if (out_y) put(row_of(static_cast<T*>(a.dy), a.ld_dy, r), j, o);
@@ -521,8 +524,8 @@ cudaError_t grad_rows_launch(const ResidualNormGradArgs& a, const GradRows& p, c
   return cudaGetLastError();
 }
 
-// Row means: stat[row] = {r2^3 A / D, r1^3 (B - r2^3 (A / D) C) / D} (the second r1-free
-// without w_post: 0).
+// Row means: stat[row] = {r2 A / D, beta r1 (B - r2 (A / D) C) / D}, which multiply v^ and y^
+// (the second is 0 without w_post).
 template <typename T, bool ANY>
 __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradArgs a, float2* stat) {
   __shared__ float red[3 * 32];
@@ -549,6 +552,7 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradAr
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] *= w[i];
+        v[i] *= r2;
         s[0] = fmaf(p[i], v[i], s[0]);
       }
     }
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradAr
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float qy = w[i] * y[i];
+        const float qy = w[i] * (y[i] * r1);
         s[1] = fmaf(qy, fmaf(r2, p[i], d[i]), s[1]);
         s[2] = fmaf(qy, v[i], s[2]);
       }
@@ -574,8 +578,8 @@ __global__ void __launch_bounds__(256) grad_stat_kernel(const ResidualNormGradAr
   row_sum(s, red);
   if (threadIdx.x == 0) {
     const float m = 1.0f / (float)a.cols;
-    const float c2 = r2 * r2 * r2 * s[0] * m;
-    stat[row] = make_float2(c2, r1 * r1 * r1 * a.beta * (s[1] - c2 * s[2]) * m);
+    const float c2 = r2 * (s[0] * m);
+    stat[row] = make_float2(c2, r1 * ((s[1] - c2 * s[2]) * m * a.beta));
   }
 }
 
@@ -672,8 +676,9 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
         get(a.v, r, a.ld_v, a.rows, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          dv[i] += r2 * wq[i] * dh[i] - v[i] * st.x;
-          dwq[i] = fmaf(dh[i], v[i] * r2, dwq[i]);
+          v[i] *= r2;
+          dv[i] += r2 * (wq[i] * dh[i]) - v[i] * st.x;
+          dwq[i] = fmaf(dh[i], v[i], dwq[i]);
         }
       }
       float o[8];
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(256) grad_cols_kernel(const ResidualNormGradAr
           const float bd = a.beta * dv[i], yh = y[i] * r1s, dz = bd * g[i];
           dg[i] = fmaf(bd * wp[i], yh, dg[i]);
           dwp[i] = fmaf(dz, yh, dwp[i]);
-          o[i] = r1s * wp[i] * dz - y[i] * st.y;
+          o[i] = r1s * wp[i] * dz - yh * st.y;
         }
         if (a.dy) put(a.dy, r, a.ld_dy, o);
       }

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import linear_ops_ref as ref
-from test_linear_ops_gpu import FMT, TYPE, check_cast, code_buffers, dev, rounded
+from test_linear_ops_gpu import FMT, TINY, TYPE, ULP, check_cast, code_buffers, dev, grad_bounds, host, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,34 @@ def test_stochastic_cast_of_fp32_next_to_each_step(engine, fmt):
     c, sf = code_buffers(fmt, *x.shape)
     engine.quantize_block(FMT[fmt], dev(x, torch.float32), c, sf, rand=dev(r, torch.uint8, fill=0))
     check_cast(c, sf, x, fmt, r)
+
+
+# ------------------------------------------------------------------ the gradient
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("size_v,size_y", [(1e13, 1e13), (1e15, 1e-3), (1e-3, 1e15), (1e16, 1e16), (1e-14, 1e-14),
+                                           (1e-18, 1e17)])
+@pytest.mark.parametrize("rows,cols", [(12, 200), (12, 1001), (3, 9000)])
+def test_norm_gradient_of_rows_of_any_magnitude(engine, typ, size_v, size_y, rows, cols):
+    # the rows' projections are of the same size as the rest of dx and dy; epsilon 0
+    rng = np.random.default_rng(72)
+    a = {"y": size_y * (1 + rng.random((rows, cols))), "w_post": 1 + 0.2 * rng.normal(size=cols),
+         "w_pre": 1 + 0.2 * rng.normal(size=cols), "gate": 1 + 0.2 * rng.normal(size=(rows, cols))}
+    a = {k: rounded(m, typ) for k, m in a.items()}
+    v = rounded(size_v * (1 + rng.random((rows, cols))), typ)
+    r1, r2 = (rounded((m * m).mean(1) ** -0.5, "f32") for m in (a["y"], v))
+    dh = rounded(1 + 0.1 * rng.normal(size=(rows, cols)), typ)
+    dxo = rounded((1 + 0.1 * rng.normal(size=(rows, cols))) / size_v, typ)
+    want = ref.norm_backward(dh, dxo, v, r2, a["w_pre"], a["y"], r1, a["w_post"], a["gate"], 1)
+    bound = grad_bounds(a, v, dh, dxo, r1, r2, 1, 1.0, 1.0, typ, cols, rows)
+    dt = TYPE[typ]
+    w1, w2, g = (torch.as_tensor(a[k]).to(dt).cuda() for k in ("w_post", "w_pre", "gate"))
+    f1, f2 = (torch.as_tensor(r).float().cuda() for r in (r1, r2))
+    out = {k: dev(np.zeros((rows, cols)), dt) for k in ("dx", "dy")}
+    out.update({k: torch.full(want[k].shape, float("nan"), device="cuda") for k in ("dgate", "dw_post", "dw_pre")})
+    engine.residual_norm_backward(
+        dev(dh, dt), dev(v, dt), f2, w2, out["dx"], dx_out=dev(dxo, dt), y=dev(a["y"], dt), rstd_post=f1,
+        w_post=w1, gate=g, dy=out["dy"], dgate=out["dgate"], dw_post=out["dw_post"], dw_pre=out["dw_pre"])
+    for k, b in bound.items():
+        if k in ("dx", "dy"):
+            b = b + ULP[typ] * (np.abs(want[k]) + b) + TINY[typ]
+        assert np.all(np.abs(host(out[k]) - want[k]) <= b), k
