@@ -58,7 +58,8 @@ b2g_status grow(b2g_handle* h, size_t bytes, size_t words, cudaStream_t s) {
     h->op_count = nullptr;
     h->op_count_words = 0;
     B2G_CUDA(h, cudaMalloc(&h->op_count, words * sizeof(uint32_t)));
-    B2G_CUDA(h, cudaMemset(h->op_count, 0, words * sizeof(uint32_t)));
+    // on the call's stream: nothing orders another one before the kernel that counts here
+    B2G_CUDA(h, cudaMemsetAsync(h->op_count, 0, words * sizeof(uint32_t), s));
     h->op_count_words = words;
   }
   return B2G_OK;
