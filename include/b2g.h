@@ -432,9 +432,10 @@ B2G_API b2g_status b2g_trace_read(const b2g_handle* h, uint32_t* out, int nwords
  * B2G_FMT_MXF4 and B2G_FMT_MXF8, in the layout b2g_gemm reads.  Matrices are
  * row-major with a leading dimension in elements; elements of a row are contiguous.
  * b2g_residual_norm_backward and b2g_linear use the handle's workspace: calls of one
- * handle on different streams must not overlap.  A workspace grows on the first call
- * that needs more (which synchronises the stream), so make such a call before a
- * stream capture. */
+ * handle on different streams must not overlap, nor must replays of graphs captured from
+ * them.  A workspace grows on a call that needs more, which synchronises the stream unless
+ * it is being captured; what a captured graph may use is kept until b2g_destroy, so a
+ * handle outlives its graphs. */
 
 typedef enum b2g_dtype { B2G_F32 = 0, B2G_BF16 = 1, B2G_F16 = 2 } b2g_dtype;
 

@@ -100,8 +100,13 @@ b2g_status b2g_destroy(b2g_handle* h) {
     if (h->d_probe) cudaFree(h->d_probe);
     if (h->part_ws) cudaFree(h->part_ws);
     if (h->flag_ws) cudaFree(h->flag_ws);
-    if (h->op_ws) cudaFree(h->op_ws);
-    if (h->op_count) cudaFree(h->op_count);
+    for (DeviceWs* w : {&h->op_ws, &h->op_count})
+      if (w->p) cudaFree(w->p);
+    while (RetiredWs* old = h->retired) {
+      h->retired = old->next;
+      cudaFree(old->p);
+      delete old;
+    }
     if (h->pipe_ready) {
       cudaStreamSynchronize(h->s_in);
       cudaStreamSynchronize(h->s_out);

@@ -7,6 +7,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <new>
+
 #include "b2g.h"
 
 typedef CUresult (*PFN_encodeTiled_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -18,6 +20,19 @@ typedef CUresult (*PFN_encodeTiled_t)(CUtensorMap*, CUtensorMapDataType, cuuint3
 // kHostColChunks column chunks
 constexpr int kHostChunks = 4;
 constexpr int kHostColChunks = 4;
+
+// A device buffer of the handle that grows on demand (reserve()).
+struct DeviceWs {
+  void* p;
+  size_t bytes;
+  bool in_graph;  // a captured graph may hold its address
+};
+
+// A buffer that was replaced while a captured graph may still use it; freed with the handle.
+struct RetiredWs {
+  void* p;
+  RetiredWs* next;
+};
 
 struct b2g_handle {
   int device;
@@ -55,10 +70,8 @@ struct b2g_handle {
   int n_occ;
   // operators around the linear layer (op_api.cu): fp32 partial sums and laid-out
   // operands of one call, and arrival counters that every launch leaves at zero
-  void* op_ws;
-  size_t op_ws_bytes;
-  uint32_t* op_count;
-  size_t op_count_words;
+  DeviceWs op_ws, op_count;
+  RetiredWs* retired;
   char last_error[512];
 };
 
@@ -91,3 +104,57 @@ struct DeviceGuard {
     if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
   }
 };
+
+// Lets the calling thread allocate while a stream is being captured.
+struct AllowInCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  AllowInCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~AllowInCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Makes w hold `bytes` bytes for a call on stream s; new ones are zeros where `zeroed`.  A
+// buffer that a captured graph may use is not freed before the handle: the graph is replayed
+// with its address.  Within a capture a larger one is allocated and zeroed at once, beside the
+// graph; outside, s is waited for, since earlier calls may still use the old one.
+inline b2g_status reserve(b2g_handle* h, DeviceWs* w, size_t bytes, bool zeroed, cudaStream_t s) {
+  if (bytes == 0) return B2G_OK;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  B2G_CUDA(h, cudaStreamIsCapturing(s, &status));
+  const bool capturing = status != cudaStreamCaptureStatusNone;
+  if (w->bytes < bytes) {
+    AllowInCapture allow;
+    if (!capturing) B2G_CUDA(h, cudaStreamSynchronize(s));
+    if (w->p && (capturing || w->in_graph)) {
+      RetiredWs* old = new (std::nothrow) RetiredWs{w->p, h->retired};
+      if (!old) return fail(h, B2G_ERR_CUDA, "out of host memory");
+      h->retired = old;
+    } else if (w->p) {
+      cudaFree(w->p);
+    }
+    *w = DeviceWs{};
+    void* p = nullptr;
+    B2G_CUDA(h, cudaMalloc(&p, bytes));
+    cudaError_t e = cudaSuccess;
+    if (zeroed && capturing) {
+      cudaStream_t beside;
+      e = cudaStreamCreateWithFlags(&beside, cudaStreamNonBlocking);
+      if (e == cudaSuccess) {
+        e = cudaMemsetAsync(p, 0, bytes, beside);
+        const cudaError_t done = cudaStreamSynchronize(beside);
+        if (e == cudaSuccess) e = done;
+        cudaStreamDestroy(beside);
+      }
+    } else if (zeroed) {
+      // on the call's stream: nothing orders another one before its kernel
+      e = cudaMemsetAsync(p, 0, bytes, s);
+    }
+    if (e != cudaSuccess) {
+      cudaFree(p);
+      return fail(h, B2G_ERR_CUDA, "zeroing a workspace failed: %s", cudaGetErrorString(e));
+    }
+    w->p = p;
+    w->bytes = bytes;
+  }
+  w->in_graph |= capturing;
+  return B2G_OK;
+}

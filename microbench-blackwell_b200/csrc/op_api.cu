@@ -43,28 +43,6 @@ bool rows_aligned(const void* p, int64_t ld, size_t elem, size_t bytes) {
   return aligned(p, bytes) && ((size_t)ld * elem) % bytes == 0;
 }
 
-b2g_status grow(b2g_handle* h, size_t bytes, size_t words, cudaStream_t s) {
-  if (h->op_ws_bytes >= bytes && h->op_count_words >= words) return B2G_OK;
-  B2G_CUDA(h, cudaStreamSynchronize(s));
-  if (h->op_ws_bytes < bytes) {
-    if (h->op_ws) cudaFree(h->op_ws);
-    h->op_ws = nullptr;
-    h->op_ws_bytes = 0;
-    B2G_CUDA(h, cudaMalloc(&h->op_ws, bytes));
-    h->op_ws_bytes = bytes;
-  }
-  if (h->op_count_words < words) {
-    if (h->op_count) cudaFree(h->op_count);
-    h->op_count = nullptr;
-    h->op_count_words = 0;
-    B2G_CUDA(h, cudaMalloc(&h->op_count, words * sizeof(uint32_t)));
-    // on the call's stream: nothing orders another one before the kernel that counts here
-    B2G_CUDA(h, cudaMemsetAsync(h->op_count, 0, words * sizeof(uint32_t), s));
-    h->op_count_words = words;
-  }
-  return B2G_OK;
-}
-
 // 128-byte swizzled map of a row-major matrix whose rows follow one another.
 b2g_status tensor_map(b2g_handle* h, CUtensorMap* map, CUtensorMapDataType type, int elem,
                       const void* base, uint64_t cols, uint64_t rows, uint32_t box_cols,
@@ -333,9 +311,9 @@ b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_norm_gra
   a.vec = fits(16);
   a.dgate_vec = aligned(d->dgate, 16);
   a.err = h->d_err;
-  const b2g_status st = grow(h, norm_grad_ws_bytes(type, a, h->sm_count), 0, s);
+  const b2g_status st = reserve(h, &h->op_ws, norm_grad_ws_bytes(type, a, h->sm_count), false, s);
   if (st != B2G_OK) return st;
-  a.ws = h->op_ws;
+  a.ws = h->op_ws.p;
   B2G_CUDA(h, launch_residual_norm_grad(type, a, h->sm_count, s));
   return B2G_OK;
 }
@@ -378,13 +356,15 @@ b2g_status b2g_linear(b2g_handle* h, const b2g_linear_desc* d, void* stream) {
   a.err = h->d_err;
   a.wait_ns = h->wait_ns;
   const bool tiles = linear_tiles(a);
-  const b2g_status st = tiles ? grow(h, few_tiles_ws_bytes(fmt, a, h->sm_count),
-                                     few_tiles_counters(fmt, a, h->sm_count), s)
-                              : grow(h, few_linear_ws_bytes(fmt, a, h->sm_count),
-                                     few_linear_counters(fmt, a, h->sm_count), s);
+  b2g_status st = reserve(h, &h->op_ws, tiles ? few_tiles_ws_bytes(fmt, a, h->sm_count)
+                                              : few_linear_ws_bytes(fmt, a, h->sm_count), false, s);
   if (st != B2G_OK) return st;
-  a.ws = h->op_ws;
-  a.count = h->op_count;
+  const size_t counters = tiles ? few_tiles_counters(fmt, a, h->sm_count)
+                                : few_linear_counters(fmt, a, h->sm_count);
+  st = reserve(h, &h->op_count, counters * sizeof(uint32_t), true, s);
+  if (st != B2G_OK) return st;
+  a.ws = h->op_ws.p;
+  a.count = static_cast<uint32_t*>(h->op_count.p);
   if (!tiles) {
     B2G_CUDA(h, launch_few_linear(fmt, d->type, a, h->sm_count, s));
     return B2G_OK;
