@@ -95,12 +95,8 @@ b2g_status b2g_destroy(b2g_handle* h) {
     DeviceGuard g(h->device);
     cudaFree(h->d_err);
     if (h->ws) cudaFree(h->ws);
-    if (h->meta_ws) cudaFree(h->meta_ws);
-    if (h->sf_ws) cudaFree(h->sf_ws);
     if (h->d_probe) cudaFree(h->d_probe);
-    if (h->part_ws) cudaFree(h->part_ws);
-    if (h->flag_ws) cudaFree(h->flag_ws);
-    for (DeviceWs* w : {&h->op_ws, &h->op_count})
+    for (DeviceWs* w : {&h->meta_ws, &h->sf_ws, &h->part_ws, &h->flag_ws, &h->op_ws, &h->op_count})
       if (w->p) cudaFree(w->p);
     while (RetiredWs* old = h->retired) {
       h->retired = old->next;
@@ -666,17 +662,11 @@ b2g_status b2g_gemm(b2g_handle* h, const b2g_gemm_desc* d, void* stream) {
     const void* ready = d->meta;
     if (d->meta_layout == 0) {
       const size_t need = meta_ready_bytes(d->M, meta_k, meta_bits);
-      if (h->meta_ws_bytes < need) {
-        B2G_CUDA(h, cudaStreamSynchronize(s));
-        if (h->meta_ws) cudaFree(h->meta_ws);
-        h->meta_ws = nullptr;
-        h->meta_ws_bytes = 0;
-        B2G_CUDA(h, cudaMalloc(&h->meta_ws, need));
-        h->meta_ws_bytes = need;
-      }
-      B2G_CUDA(h, launch_meta_ready((const uint32_t*)d->meta, d->M, meta_k, (uint32_t*)h->meta_ws,
+      st = reserve(h, &h->meta_ws, need, false, s);
+      if (st != B2G_OK) return st;
+      B2G_CUDA(h, launch_meta_ready((const uint32_t*)d->meta, d->M, meta_k, (uint32_t*)h->meta_ws.p,
                                     h->sm_count, s, meta_bits));
-      ready = h->meta_ws;
+      ready = h->meta_ws.p;
     }
     // one box per ring slot and 128-row block: 2 KB (16-bit A) or 4 KB (8-bit), in
     // kSideLine-byte lines
@@ -699,15 +689,9 @@ b2g_status b2g_gemm(b2g_handle* h, const b2g_gemm_desc* d, void* stream) {
     const size_t na = sf_ready_bytes(d->M, sf_cols, groups, 128, 128);
     const size_t nb = sf_ready_bytes(d->N, sf_cols, groups, bn, 256);
     const size_t need = na + nb;
-    if (h->sf_ws_bytes < need) {
-      B2G_CUDA(h, cudaStreamSynchronize(s));
-      if (h->sf_ws) cudaFree(h->sf_ws);
-      h->sf_ws = nullptr;
-      h->sf_ws_bytes = 0;
-      B2G_CUDA(h, cudaMalloc(&h->sf_ws, need));
-      h->sf_ws_bytes = need;
-    }
-    uint8_t* ra = static_cast<uint8_t*>(h->sf_ws);
+    st = reserve(h, &h->sf_ws, need, false, s);
+    if (st != B2G_OK) return st;
+    uint8_t* ra = static_cast<uint8_t*>(h->sf_ws.p);
     uint8_t* rb = ra + na;
     B2G_CUDA(h, launch_sf_ready(sf_ready(d->sfa, d->M, sf_cols, 128, 128, ra),
                                 sf_ready(d->sfb, d->N, sf_cols, bn, 256, rb), sf_cols, groups,
@@ -760,27 +744,12 @@ b2g_status b2g_gemm(b2g_handle* h, const b2g_gemm_desc* d, void* stream) {
     const int rem = tiles - p.pub.tail_start;
     const size_t part_need = (size_t)rem * (S - 1) * (size_t)(128 * cg) * (size_t)bn * sizeof(float);
     const size_t flag_need = (size_t)rem * (S - 1) * cg * 4 * sizeof(uint32_t);
-    if (h->part_ws_bytes < part_need || h->flag_ws_bytes < flag_need) {
-      B2G_CUDA(h, cudaStreamSynchronize(s));
-      if (h->part_ws_bytes < part_need) {
-        if (h->part_ws) cudaFree(h->part_ws);
-        h->part_ws = nullptr;
-        h->part_ws_bytes = 0;
-        B2G_CUDA(h, cudaMalloc(&h->part_ws, part_need));
-        h->part_ws_bytes = part_need;
-      }
-      if (h->flag_ws_bytes < flag_need) {
-        if (h->flag_ws) cudaFree(h->flag_ws);
-        h->flag_ws = nullptr;
-        h->flag_ws_bytes = 0;
-        B2G_CUDA(h, cudaMalloc(&h->flag_ws, flag_need));
-        B2G_CUDA(h, cudaMemset(h->flag_ws, 0, flag_need));
-        h->flag_ws_bytes = flag_need;
-      }
-    }
+    st = reserve(h, &h->part_ws, part_need, false, s);
+    if (st == B2G_OK) st = reserve(h, &h->flag_ws, flag_need, true, s);
+    if (st != B2G_OK) return st;
     if (++h->epoch == 0) ++h->epoch;  // 0 is the value of fresh flags
-    a.part = static_cast<float*>(h->part_ws);
-    a.flags = h->flag_ws;
+    a.part = static_cast<float*>(h->part_ws.p);
+    a.flags = static_cast<uint32_t*>(h->flag_ws.p);
     a.epoch = h->epoch;
   }
   const int clusters = p.pub.clusters;

@@ -43,15 +43,11 @@ struct b2g_handle {
   PFN_encodeTiled_t encode_tiled;
   void* ws;                // device workspace of b2g_gemm_host
   size_t ws_bytes;
-  void* meta_ws;           // scratch: engine-layout 2:4 metadata of the last sparse call
-  size_t meta_ws_bytes;
-  void* sf_ws;             // scratch: engine-layout NVFP4 scale factors of the last call
-  size_t sf_ws_bytes;
+  DeviceWs meta_ws;        // scratch: engine-layout 2:4 metadata of the last sparse call
+  DeviceWs sf_ws;          // scratch: engine-layout scale factors of the last call
   void* d_probe;           // b2g_probe_mma result words
-  void* part_ws;           // split tail: fp32 partial tiles
-  size_t part_ws_bytes;
-  uint32_t* flag_ws;       // split tail: per-warp stamps (zeroed when allocated)
-  size_t flag_ws_bytes;
+  DeviceWs part_ws;        // split tail: fp32 partial tiles
+  DeviceWs flag_ws;        // split tail: per-warp stamps (zeroed when allocated)
   uint32_t epoch;          // stamp of the last split-tail launch
   uint64_t wait_ns;        // limit of the kernel-side bounded waits (0: kWaitLimitNs)
   // b2g_gemm_host pipeline: copy-in and copy-out streams, events per row chunk
