@@ -747,6 +747,12 @@ b2g_status b2g_gemm(b2g_handle* h, const b2g_gemm_desc* d, void* stream) {
     st = reserve(h, &h->part_ws, part_need, false, s);
     if (st == B2G_OK) st = reserve(h, &h->flag_ws, flag_need, true, s);
     if (st != B2G_OK) return st;
+    // A graph launches its kernel with the same epoch every time: it clears the stamps that its
+    // last replay left before the kernel waits for them.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    B2G_CUDA(h, cudaStreamIsCapturing(s, &capture));
+    if (capture != cudaStreamCaptureStatusNone)
+      B2G_CUDA(h, cudaMemsetAsync(h->flag_ws.p, 0, flag_need, s));
     if (++h->epoch == 0) ++h->epoch;  // 0 is the value of fresh flags
     a.part = static_cast<float*>(h->part_ws.p);
     a.flags = static_cast<uint32_t*>(h->flag_ws.p);

@@ -55,3 +55,23 @@ def test_graphs_outlive_the_growth_of_the_workspaces(engine, fresh):
         assert torch.equal(out, want)
     assert all((r == 0xFF).all() for r in rubbish)
     fresh.check()
+
+
+@pytest.mark.parametrize("M,N,K", [(500, 1024, 2048), (512, 512, 8192), (2500, 2048, 2048)])
+def test_replays_of_a_split_tail_use_their_own_partial_sums(engine, fresh, M, N, K):
+    # every replay has other inputs: sums that the last one left would show
+    assert b2g.plan_gemm(b2g.FMT_BF16, M, N, K)["tail_split"] > 1
+    a, b = (torch.empty(r, K, dtype=torch.bfloat16, device="cuda") for r in (M, N))
+    out, want = (torch.empty(M, N, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    graph = captured(lambda: [fresh.gemm(a, b, out, b2g.FMT_BF16) for _ in range(2)])
+    g = torch.Generator(device="cuda").manual_seed(11)
+    for _ in range(6):
+        for t in (a, b):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        engine.gemm(a, b, want, b2g.FMT_BF16)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        fresh.gemm(a, b, out, b2g.FMT_BF16)
+        assert torch.equal(out, want)
+    fresh.check()
