@@ -7,20 +7,24 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 namespace b2g {
 
 // Lets a kernel use `bytes` of dynamic shared memory on the current device.  The attribute
 // is set once for each kernel, device and size above the last (`seen`: one word per device,
-// the kernel's own).
+// the kernel's own), by one host thread at a time: a smaller size may not come behind a larger.
 template <typename K>
 inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<int> (&seen)[16]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 16 && seen[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  static std::mutex one;
+  std::lock_guard<std::mutex> lock(one);
   if (dev < 16 && seen[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 16) seen[dev].store(bytes, std::memory_order_relaxed);
+  if (e == cudaSuccess && dev < 16) seen[dev].store(bytes, std::memory_order_release);
   return e;
 }
 
