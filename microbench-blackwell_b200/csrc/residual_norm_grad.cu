@@ -42,6 +42,16 @@ struct GradRows {
   size_t smem;
 };
 
+// Shared memory of a CTA: slots for a row's four or five tensors; any alignment: 32 bytes more a
+// tensor, and a buffer for each warp's stores.
+constexpr size_t kGradRoom = 224 * 1024;
+constexpr size_t grad_stage(int max_threads, int nv, int elem, bool few) {
+  return (size_t)max_threads * nv * (few ? 5 : 4) * 8 * elem;
+}
+constexpr size_t grad_smem(int stages, size_t stage, int max_threads, bool any) {
+  return stages * (stage + (any ? 5 * 32 : 0)) + (any ? max_threads / 32 * 65 * 16 : 0);
+}
+
 // What is summed over rows that more than one CTA has: part[cta][2][cols] (dw_pre, dw_post)
 // and slots[2 cta + (0: the gate the CTA starts in, 1: the one it ends in)][cols].
 __device__ __host__ __forceinline__ int64_t first_row(int64_t cta, int64_t rows, int64_t ctas) {
@@ -459,16 +469,14 @@ GradRows grad_rows(int type, const ResidualNormGradArgs& a, int sm_count) {
   p.max_threads = threads > 256 ? 512 : threads > 128 ? 256 : 128;
   // FEW; a gate per 4 rows of 8192 485 us so, 559 without, per 7 of 4096 265 and 259
   p.gate_rows = a.gate && a.rows_per_gate < 8 && a.rows_per_gate < a.rows;
-  const size_t stage = (size_t)p.max_threads * p.nv * (p.gate_rows ? 5 : 4) * 8 * es;
+  const size_t stage = grad_stage(p.max_threads, p.nv, es, p.gate_rows);
   // CTAs on an SM: by registers (128 a thread) and shared memory
-  const size_t room = 224 * 1024;
   int on_sm = 512 / p.max_threads;
   p.stages = kRowStages;
-  if (!p.any && p.stages * stage * on_sm > room) p.stages = 2;
-  // any alignment: 32 bytes more a tensor, and a buffer for each warp's stores
-  p.smem = p.stages * (stage + (p.any ? 5 * 32 : 0)) + (p.any ? p.max_threads / 32 * 65 * 16 : 0);
-  while (on_sm > 1 && p.smem * on_sm > room) --on_sm;
-  if (p.smem > room) return p;
+  if (!p.any && p.stages * stage * on_sm > kGradRoom) p.stages = 2;
+  p.smem = grad_smem(p.stages, stage, p.max_threads, p.any);
+  while (on_sm > 1 && p.smem * on_sm > kGradRoom) --on_sm;
+  if (p.smem > kGradRoom) return p;
   const int64_t most = (int64_t)on_sm * sm_count;
   // at least two rows a CTA: each costs its sums' way through memory
   const int64_t want = (a.rows + 1) / 2;
@@ -480,11 +488,18 @@ GradRows grad_rows(int type, const ResidualNormGradArgs& a, int sm_count) {
 template <typename T, int NV, int MAXT, bool ALL, bool FEW, bool ANY>
 cudaError_t grad_rows_main(const ResidualNormGradArgs& a, const GradRows& p, float* part, float* slots,
                            cudaStream_t s) {
-  static std::atomic<int> seen[16];
-  const cudaError_t e = allow_smem(grad_rows_kernel<T, NV, MAXT, ALL, FEW, ANY>, (int)p.smem, seen);
-  if (e != cudaSuccess) return e;
-  grad_rows_kernel<T, NV, MAXT, ALL, FEW, ANY><<<p.ctas, p.threads, p.smem, s>>>(a, p, part, slots);
-  return cudaGetLastError();
+  // grad_rows() chooses no form whose slots do not fit
+  constexpr size_t least =
+      grad_smem(ANY ? kRowStages : 2, grad_stage(MAXT, NV, sizeof(T), FEW), MAXT, ANY);
+  if constexpr (least > kGradRoom) {
+    return cudaErrorInvalidConfiguration;
+  } else {
+    static std::atomic<int> seen[16];
+    const cudaError_t e = allow_smem(grad_rows_kernel<T, NV, MAXT, ALL, FEW, ANY>, (int)p.smem, seen);
+    if (e != cudaSuccess) return e;
+    grad_rows_kernel<T, NV, MAXT, ALL, FEW, ANY><<<p.ctas, p.threads, p.smem, s>>>(a, p, part, slots);
+    return cudaGetLastError();
+  }
 }
 
 template <typename T, bool ALL, bool FEW, bool ANY>

@@ -6,6 +6,7 @@ import torch
 
 import linear_ops_ref as ref
 from test_linear_ops_gpu import FMT, TINY, TYPE, ULP, check_cast, code_buffers, dev, grad_bounds, host, rounded
+from test_linear_ops_gpu import test_norm_gradient as check_gradient
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +154,12 @@ def test_norm_gradient_of_rows_of_any_magnitude(engine, typ, size_v, size_y, row
         if k in ("dx", "dy"):
             b = b + ULP[typ] * (np.abs(want[k]) + b) + TINY[typ]
         assert np.all(np.abs(host(out[k]) - want[k]) <= b), k
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,per", [(20, 2056, 3), (20, 4096, 3), (20, 4097, 3), (24, 8192, 4), (9, 8191, 2),
+                                           (9, 8184, 9), (5, 8200, 1)])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_norm_gradient_where_its_forms_change(engine, typ, rows, cols, per, pad):
+    # one pass or two, by columns, type, alignment and the rows of a gate
+    check_gradient(engine, typ, rows, cols, per, pad)
