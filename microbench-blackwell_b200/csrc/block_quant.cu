@@ -91,12 +91,12 @@ __device__ __forceinline__ Rand16 load_rand16(const BlockQuantArgs& a, const uin
   return r;
 }
 
-template <int FMT, int QM, bool SR>
+template <int FMT, int QM, bool SR, bool FOLD>
 __device__ __forceinline__ void store_row16(const float2 (&x)[2][4], const BlockScale& s, float fold,
                                             const Rand16& rnd, uint8_t* codes, uint8_t* sf) {
   uint32_t lo[2], hi[2];
-  encode8<FMT, QM, SR>(x[0], s, fold, rnd.h[0], lo);
-  encode8<FMT, QM, SR>(x[1], s, fold, rnd.h[1], hi);
+  encode8<FMT, QM, SR, FOLD>(x[0], s, fold, rnd.h[0], lo);
+  encode8<FMT, QM, SR, FOLD>(x[1], s, fold, rnd.h[1], hi);
   if constexpr (FMT == BF_MXF8)
     *reinterpret_cast<uint4*>(codes) = make_uint4(lo[0], lo[1], hi[0], hi[1]);
   else
@@ -133,7 +133,7 @@ __device__ __forceinline__ void encode_row16(const Raw16<T>& raw, float scale, c
   }
   if constexpr (bf_block(FMT) == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
   const BlockScale s = block_scale<FMT, QM>(amax);
-  if (write) store_row16<FMT, QM, SR>(x, s, PRE ? 1.0f : scale, rnd, codes, sf);
+  if (write) store_row16<FMT, QM, SR, !PRE>(x, s, scale, rnd, codes, sf);
 }
 
 // Rows only: 16 elements per thread (a block of NVFP4, so that its scale needs no other lane;
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) quant_both_kernel(const BlockQuantAr
       rnd[1] = make_uint2(b[2], b[3]);
     }
     uint32_t lo[2], hi[2];
-    encode8<FMT, QM, SR>(y[0], s, PRE ? 1.0f : a.scale, rnd[0], lo);
-    encode8<FMT, QM, SR>(y[1], s, PRE ? 1.0f : a.scale, rnd[1], hi);
+    encode8<FMT, QM, SR, !PRE>(y[0], s, a.scale, rnd[0], lo);
+    encode8<FMT, QM, SR, !PRE>(y[1], s, a.scale, rnd[1], hi);
     if (c < a.cols && r < a.tp) {
       uint8_t* dst = a.codes_t + (c * a.tp + r) * bits / 8;
       if constexpr (FMT == BF_MXF8)

@@ -458,18 +458,18 @@ __device__ __forceinline__ float round_stochastic(float x, const BlockScale& s,
   return __uint_as_float(bits) * __uint_as_float((__float_as_uint(x) & 0x80000000u) | __float_as_uint(up));
 }
 
-// Codes of eight elements of one block (times `fold`, a power of two): 32 bits (e2m1) in
-// w[0] or 64 (e4m3) in w[0..1].  rnd: eight random bytes, used when SR.
-template <int FMT, int QM, bool SR>
+// Codes of eight elements of one block (times `fold`, a power of two, where FOLD): 32 bits
+// (e2m1) in w[0] or 64 (e4m3) in w[0..1].  rnd: eight random bytes, used when SR.
+template <int FMT, int QM, bool SR, bool FOLD>
 __device__ __forceinline__ void encode8(const float2 (&in)[4], const BlockScale& s, float fold,
                                         uint2 rnd, uint32_t (&w)[2]) {
   float2 q[4];
-  float mult = s.inv * fold;
+  float mult = FOLD ? s.inv * fold : s.inv;
   float2 x[4] = {in[0], in[1], in[2], in[3]};
   // MX: fold / s leaves fp32's range in a block of zeros, or one so small that its scale is the
   // least or next to it.  fold then goes into the elements first: 0 * infinity would be NaN.
   // (Both ways, 8192 x 8192 bf16: 55 and 59 us; without this test 53 and 57.)
-  if (QM == Q_EXACT && mult > 0x1.fffffep127f) {
+  if (FOLD && QM == Q_EXACT && mult > 0x1.fffffep127f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], both(fold));
     mult = s.inv;

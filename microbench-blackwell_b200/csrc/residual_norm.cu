@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const ResidualNormA
       if constexpr (blk == 32) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
       const BlockScale s = block_scale<HF, mode>(amax);
       uint32_t q[2];
-      encode8<HF, mode, false>(v[j], s, 1.0f, make_uint2(0, 0), q);
+      encode8<HF, mode, false, false>(v[j], s, 1.0f, make_uint2(0, 0), q);
       if (col[j] < a.kp) {
         const int64_t e = row * a.kp + col[j];
         if constexpr (HF == BF_MXF8)
