@@ -469,7 +469,8 @@ typedef struct b2g_block_quant_desc {
 B2G_API b2g_status b2g_block_quantize(b2g_handle* h, const b2g_block_quant_desc* d, void* stream);
 
 /* Reads codes and scales in b2g_block_quantize's layout back: out[rows][cols] =
- * code * block scale * scale, rounded once to out_type. */
+ * code * block scale * scale in fp32 (exact where scale is a power of two), then rounded
+ * to out_type. */
 B2G_API b2g_status b2g_block_dequantize(b2g_handle* h, int format, const void* d_codes,
                                         const void* d_sf, int64_t rows, int64_t cols,
                                         int out_type, void* d_out, int64_t ld_out, float scale,
@@ -542,7 +543,9 @@ B2G_API b2g_status b2g_residual_norm_backward(b2g_handle* h, const b2g_residual_
 /* out[T][N] = alpha * x[T][K] . W[N][K]^T for the few tokens of a decode step: x and
  * out bf16 or fp16, W as codes and scales in b2g_block_quantize's layout ([N][Kp], Kp =
  * K rounded up to 32, padding zero), x not cast: fp32 sums of products of x and the
- * weights' values.  An infinity or a NaN in x makes the outputs of its token infinite or
+ * weights' values.  bf16 x is held as fp16 times a power of two for each token: exact for
+ * values down to 2^-28 of the token's largest, within 2^-40 of it below, and sums overflow
+ * where the weights of a row add up to more than 2^112.  An infinity or a NaN in x makes the outputs of its token infinite or
  * NaN.  Reads the weights once for every 128 tokens; for many tokens cast x and use
  * b2g_gemm.  w 16-byte, sfw 2-byte aligned.  From nine tokens on a kernel wait that ran
  * out is reported by b2g_check, as for b2g_gemm. */

@@ -6,10 +6,10 @@
 // each operand twice, because the products of forward and backward run along different
 // dimensions and a block's scale lies along the product's.
 //
-// Bound by bytes along the rows: 8192 x 8192 bf16 into NVFP4 29 us (5.9 TB/s of 6.5 measured
-// by a copy), MXFP4 27, MXFP8 31, read back 32 to 35.  Both ways in one pass 52, 47 and 52 us
-// (rows alone and columns alone 66, 63 and 69) and rounded by given bytes 85, 80 and 86: there
-// the conversions bound it.  Rows off 16 bytes (8190 columns) 40, 33 and 35 us along the rows.
+// Bound by bytes along the rows: 8192 x 8192 bf16 into NVFP4 27 us (6.3 TB/s of 6.5 measured
+// by a copy), MXFP4 27, MXFP8 31, read back 34 to 38.  Both ways in one pass 50, 50 and 53 us
+// (rows alone and columns alone 64, 64 and 69) and rounded by given bytes 83, 82 and 86: there
+// the conversions bound it.  Rows off 16 bytes (8190 columns) 37, 37 and 39 us along the rows.
 #include "b2g.h"
 #include "op_common.cuh"
 #include "op_kernels.h"
@@ -137,7 +137,7 @@ __device__ __forceinline__ void encode_row16(const Raw16<T>& raw, float scale, c
 }
 
 // Rows only: 16 elements per thread (a block of NVFP4, so that its scale needs no other lane;
-// eight a thread took 45 us where this takes 29).  blockDim.x threads along a row, blockDim.y
+// eight a thread took 45 us where this took 29).  blockDim.x threads along a row, blockDim.y
 // rows.
 template <typename T, int FMT, int QM, bool SR, bool PRE>
 __global__ void __launch_bounds__(kThreads) quant_rows_kernel(const BlockQuantArgs a) {
@@ -451,8 +451,8 @@ cudaError_t quant_sr(const BlockQuantArgs& a, cudaStream_t s) {
 
 // PRE: each element is multiplied by `scale` first.  16-bit inputs with a power of two need
 // not: it goes into the reciprocal of the block's scale, and NVFP4 quotients are then found
-// without a division (8192 x 8192 bf16 into NVFP4 along the rows: scale 1 29 us, scale 3 48 us;
-// both ways 52 and 99 us).
+// without a division (8192 x 8192 bf16 into NVFP4 along the rows: scale 1 27 us, scale 3 48 us;
+// both ways 50 and 100 us).
 template <typename T>
 cudaError_t quant_fmt(int fmt, bool pow2, const BlockQuantArgs& a, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {

@@ -7,8 +7,8 @@
 // by a first kernel, is operand B, up to 128 tokens of it; sums stay in tensor memory until
 // the end.  A decoded weight then serves all tokens for one instruction's issue.
 //
-// Measured, 16384 x 8192, 16 tokens: NVFP4 21.4 us, MXFP4 23.3, MXFP8 34.3; 64 tokens 25.7,
-// 28.5, 37.9; 128 tokens 43.6, 46.4, 47.3 (x is read from L2 by every CTA, 64 KB for each
+// Measured, 16384 x 8192, 16 tokens: NVFP4 21.4 us, MXFP4 23.3, MXFP8 34.0; 64 tokens 25.5,
+// 28.3, 37.1; 128 tokens 43.0, 46.0, 46.9 (x is read from L2 by every CTA, 64 KB for each
 // 16 KB of codes); 2048 x 2048, 16 tokens 8 to 9 us.  Of MXFP4's 16 tokens about 6 us pass
 // before the first step is decoded (x's layout, launch, first copies) and 2 after the last;
 // between, a step of 256 elements x 128 rows takes 0.43 us, 4.9 TB/s of weights, MXFP8's, of half
@@ -35,7 +35,7 @@ constexpr int kQuads = kGroups * kHalves;  // sets of four warps
 constexpr int kDecodeWarps = 4 * kQuads;
 constexpr int kThreads = (kDecodeWarps + 2) * 32;
 constexpr int kCodeBytes = 128;       // of a row in a step
-constexpr int kMaxStages = 6;          // MXFP8 16384 x 8192 37.4 us with six, 40.6 with four
+constexpr int kMaxStages = 6;          // MXFP8 16384 x 8192 34.0 us with six, 38.1 with four
 constexpr int kMaxBuffers = 4;        // of decoded steps in tensor memory
 constexpr int kScaleBytes = 2048;     // of a ring slot: 16, 8 or 4 bytes a row
 

@@ -1,5 +1,5 @@
 // residual_norm.cu -- norms before and after a block, fused with its gate and residual
-// scale, and their gradient.
+// scale.
 //
 //   z = y * rstd(y) * w_post            (z = y without w_post)
 //   v = alpha * x + beta * gate * z     (v = alpha * x without y)

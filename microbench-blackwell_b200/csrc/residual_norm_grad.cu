@@ -24,12 +24,12 @@ namespace {
 
 // Rows of up to 8192 columns go through grad_rows_kernel in one pass; wider ones, which do not
 // fit a CTA's registers and shared memory, through a pass for the means and one down the
-// columns (16384 x 8192 bf16: 351 us in one pass, 905 us in two).
+// columns (16384 x 8192 bf16: 352 us in one pass, 905 us in two).
 
 // One pass: a CTA owns a run of rows and all columns, NV times eight a thread, with the
 // sums over its rows in registers.  Each thread copies its own part of the next rows into
 // shared memory while it works on one, so a row costs one barrier, for the means.
-// Reads 4 and writes 2 elements for each; 16384 x 8192 bf16 351 us, 4.6 TB/s of the 6.5 that a
+// Reads 4 and writes 2 elements for each; 16384 x 8192 bf16 352 us, 4.6 TB/s of the 6.5 that a
 // copy measures: with the column sums 128 registers a thread leave 16 warps an SM, and a row's
 // barrier and two chains of sums are not hidden by them all.  Bulk copies in place of each
 // thread's own took 364 us, 1024 threads of 64 registers 440 us.
@@ -63,10 +63,11 @@ __device__ __host__ __forceinline__ int64_t first_row(int64_t cta, int64_t rows,
 // w_post is kept as one product; both are renewed when the gate changes.
 // MAXT: bound of the CTA's threads and their stride in shared memory.  ALL: dh, dx_out, y,
 // w_post, dx and dy are there, so that the common pass is free of tests for them (16384 x 8192
-// 351 us, with the tests 372).  FEW: a gate has few rows; its values come through the ring and
-// dw_post stays in registers, where otherwise it is added up in `part` (a gate a row 525 us,
+// 352 us, with the tests 372).  FEW: a gate has few rows; its values come through the ring and
+// dw_post stays in registers, where otherwise it is added up in `part` (a gate a row 522 us,
 // without 700; a gate per 16 rows of 4096 258 us, without 246).
-// ANY: operands of any alignment (16384 x 8191 803 us, in two passes 1346).  Rows are copied as the aligned words that cover them and
+// ANY: operands of any alignment (16384 x 8191 887 us, in two passes 1346; 803 with
+// the powers of r in the row's scalars, which leave fp32's range).  Rows are copied as the aligned words that cover them and
 // shifted on the way out of shared memory; an element may then lie in a neighbour's copy,
 // so a row's copies have landed, for all, by the barrier of the row before, and its slot
 // is filled again after the barrier of the row behind.
@@ -462,8 +463,8 @@ GradRows grad_rows(int type, const ResidualNormGradArgs& a, int sm_count) {
   if (v > 1024) return p;
   p.any = !a.vec || a.cols % 8;
   const int es = type == B2G_F32 ? 4 : 2;
-  // sixteen columns a thread only where eight do not do: 32768 x 4096 354 us with sixteen, 340
-  // with eight, 65536 x 2048 431 and 310
+  // sixteen columns a thread only where eight do not do: 32768 x 4096 354 us with sixteen, 339
+  // with eight, 65536 x 2048 431 and 316
   p.nv = v > 512 ? 2 : 1;
   const int threads = ((int)((v + p.nv - 1) / p.nv) + 31) / 32 * 32;
   p.max_threads = threads > 256 ? 512 : threads > 128 ? 256 : 128;
